@@ -13,6 +13,7 @@
  */
 #ifndef MCPM_H
 #define MCPM_H
+#include <stddef.h>
 #include <stdint.h>
 
 #ifdef __cplusplus
@@ -295,6 +296,116 @@ mcpm_status mcpm_attention_noalloc(const float* q, const float* k, const float* 
 enum { MCPM_ORDER_AVX2 = 0, MCPM_ORDER_BLOCK = 1 };
 mcpm_status mcpm_gemv_q8k_timed(int type, const void* w, int n_copies, const void* xq, float* y, int rows, int cols,
                                 int order, int reps, float* ms_per_launch, void* stream);
+
+/* ------------------------------------------------------------------ paged KV cache (device pointers)
+ * No counterpart in the reference, whose cache is one contiguous array per layer
+ * (include/ops.h:147-150).  A pool holds n_pages pages of page_size positions of one layer's K
+ * and V rows; a sequence owns the pages that its row of the page table names, so sequences of
+ * unlike lengths share one memory budget, and equal prefixes can share pages.
+ *
+ * Geometry.  n_head = g * n_head_kv query heads, 1 <= g <= 16 per KV head; head_dim 64 or 128; any
+ * page_size >= 1.  Element (page, slot, kv head, dim) of K and of V lies at page * page_stride +
+ * slot * row_stride + head * head_stride + dim elements (64-bit arithmetic); all three strides 0:
+ * packed [page][slot][kv head][dim], whose rows are the engine cache's [pos][256] rows.  Strides
+ * are multiples of 16 bytes and pool pointers 16-byte aligned.  `mass`, where a pool has it:
+ * float [page][kv head][slot], the attention weight that each position has received.
+ *
+ * Page tables are int32 [n_seq][max_pages].  A page id outside [0, n_pages) is an absent page: its
+ * positions are not visible to attention, are not kept by an eviction, and rows written to it are
+ * dropped.  Lengths are int32 device values, clamped to [0, max_pages * page_size]; the host never
+ * reads them, so every call can be captured in a CUDA graph and replayed as the lengths grow.
+ *
+ * No call allocates.  `ws` is a workspace of at least mcpm_paged_workspace_bytes bytes, 16-byte
+ * aligned, zero-filled once before its first use; each call leaves it ready for the next call with
+ * the same configuration.  Calls that may overlap on the GPU need a workspace each. */
+enum { MCPM_KV_BF16 = 2 };   /* kv_type of a paged pool, beside MCPM_KV_F32 and MCPM_KV_F16 */
+typedef struct {
+    int kv_type;      /* MCPM_KV_F32, MCPM_KV_F16 or MCPM_KV_BF16: element type of K and V */
+    int n_head, n_head_kv, head_dim;
+    int page_size;    /* positions per page */
+    int n_pages;      /* pages of a pool; n_pages * page_size <= 2^30 */
+    int max_seqs;     /* most sequences of one call */
+    int max_pages;    /* columns of a page table; max_pages * page_size <= 2^30 */
+    int64_t page_stride, row_stride, head_stride;   /* elements; 0, 0, 0: packed */
+} mcpm_paged_config;
+typedef struct {
+    void* k;
+    void* v;
+    float* mass;      /* NULL: no weights are kept (append, attention) */
+} mcpm_paged_pool;
+/* Bytes of the workspace that the calls with this configuration need; 0: the configuration is invalid. */
+size_t mcpm_paged_workspace_bytes(const mcpm_paged_config* cfg);
+/* RoPE factors of positions [0, n_pos) for mcpm_paged_append: out (host) is float
+ * [n_pos][head_dim / 2][2], (cos, sin) of pos * rope_base^(-2i/head_dim), computed with the host C
+ * library as the engine's own table is. */
+mcpm_status mcpm_rope_table(float* out, int n_pos, int head_dim, float rope_base);
+typedef struct {
+    int n_tok;               /* new tokens */
+    const int* tok_seq;      /* [n_tok] row of the page table; NULL: token i belongs to row i */
+    const int* tok_slot;     /* [n_tok] place in the sequence's cache; negative: padding, nothing is written */
+    const int* tok_pos;      /* [n_tok] position that the rotation uses; NULL: tok_slot */
+    const float* q;          /* [n_tok][n_head * head_dim]; NULL: no queries */
+    float* q_out;            /* rotated queries, rows of n_head * head_dim; may be q (with q_stride n_head * head_dim) */
+    int64_t q_stride;        /* floats between the rows of q; 0: n_head * head_dim */
+    const float *k, *v;      /* [n_tok][n_head_kv * head_dim] */
+    int64_t kv_stride;       /* floats between the rows of k, and of v; 0: n_head_kv * head_dim */
+    const float* rope;       /* [rope_len][head_dim / 2][2]; NULL: q and k are rotated already */
+    int rope_len;            /* positions outside [0, rope_len) are clamped to it */
+} mcpm_paged_tokens;
+/* Appends n_tok tokens (of any sequences, any number of each: a decode step or a prompt): rotates
+ * q and k by interleaved pairs (2i, 2i+1) as mcpm_rope_kv_append does, rounds k and v to the cache
+ * type (nearest, ties to even) into slot tok_slot of sequence tok_seq, and zeroes the mass of those
+ * positions.  No two tokens of a call may name the same slot.  Rows 16-byte aligned.
+ * table: [n_seq][max_pages]; tok_seq outside [0, n_seq) is padding. */
+mcpm_status mcpm_paged_append(const mcpm_paged_config* cfg, const mcpm_paged_pool* pool, const int* table, int n_seq,
+                              const mcpm_paged_tokens* tokens, void* stream);
+/* GQA attention of one query per sequence over its pages (execute_attention, ops.cpp:537-628, on a
+ * paged cache): out_h = softmax_j(scale q_h . K_j) V over the present positions j < seq_len; a
+ * sequence that sees none gets zeros.  q and out: rows of n_head * head_dim floats, q_stride floats
+ * between the rows of q (0: packed).  scale 0: 1/sqrt(head_dim).  With pool->mass, each visible
+ * position's mass grows by the sum of its weights over the g query heads of its KV head; the
+ * sequences of such a call share no pages.  Results do not depend on how the work was split over
+ * the GPU in other calls: equal inputs give equal bits. */
+mcpm_status mcpm_paged_attention(const mcpm_paged_config* cfg, const mcpm_paged_pool* pool, const int* table,
+                                 const int* seq_len, int n_seq, const float* q, int64_t q_stride, float* out,
+                                 float scale, void* ws, size_t ws_bytes, void* stream);
+/* Eviction: for each sequence and KV head, keeps the n_keep present positions j < seq_len that come
+ * first in this order: j < n_sink or j >= seq_len - n_recent; then larger mass (NaN counts as
+ * lightest); then smaller j.  The kept rows of K and V and their masses are copied, in order of j, to
+ * places 0, 1, ... of the sequence's row of dst_table; the rows they came from stay as they are, so
+ * prefix pages of other sequences stay valid and the caller frees its own.  kept (int32
+ * [n_seq][n_head_kv][n_keep]) receives the positions, -1 beyond the last; new_len (int32 [n_seq]) the
+ * number kept: n_keep, or all present positions where they are fewer.  No page of dst_table may be
+ * one that a row of table names.  n_sink + n_recent <= n_keep <= max_pages * page_size. */
+mcpm_status mcpm_paged_evict(const mcpm_paged_config* cfg, const mcpm_paged_pool* pool, const int* table,
+                             const int* seq_len, const int* dst_table, int* new_len, int* kept, int n_seq, int n_keep,
+                             int n_sink, int n_recent, void* ws, size_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------ logits (device pointers)
+ * Penalties, biases and a grammar mask on logits, before a sampler (the reference samples the raw
+ * logits, src/sampler.cpp:8-72).  Per row, with c = the number of times that token t stands in the
+ * row's history: x = logit; where c > 0, x = (x > 0 ? x / repetition : x * repetition) - (frequency *
+ * c + presence); a biased token's x += its bias; a token whose allow bit is 0 becomes -inf. */
+typedef struct {
+    int n_seq, n_vocab;
+    const float* logits;     /* rows of n_vocab */
+    float* out;              /* may be logits */
+    int64_t logits_stride, out_stride;   /* floats between rows; 0: n_vocab */
+    const int* hist;         /* [n_seq] rows of token ids; NULL: no penalties; ids outside the vocabulary are ignored */
+    const int* hist_len;     /* [n_seq]; NULL: hist_max of each row; clamped to [0, hist_max] */
+    int hist_max;            /* tokens of a history row, <= 1048575 */
+    int64_t hist_stride;     /* ints between rows; 0: hist_max */
+    const float* penalties;  /* [n_seq][3]: repetition (> 0), frequency, presence */
+    const int* bias_token;   /* [n_seq] rows of token ids; NULL: no biases; a token listed twice takes its last entry */
+    const float* bias;
+    const int* bias_len;     /* [n_seq]; NULL: bias_max of each row; clamped to [0, bias_max] */
+    int bias_max;            /* entries of a bias row, <= 4094 */
+    int64_t bias_stride;     /* entries between rows; 0: bias_max */
+    const uint32_t* allow;   /* [n_seq] rows of (n_vocab + 31) / 32 words, bit t % 32 of word t / 32; NULL: all */
+    int64_t allow_stride;    /* words between rows; 0: (n_vocab + 31) / 32 */
+    int* argmax;             /* [n_seq], optional: the largest x, lowest token on ties, NaN never; -1: no x above -inf */
+} mcpm_logits_params;
+mcpm_status mcpm_logits_process(const mcpm_logits_params* p, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,143 @@
+// Logit processing before a sampler: penalties for repeated tokens, biases, a grammar bit mask and
+// the greedy token of the result, in one pass over the logits.
+#include <cmath>
+#include <cstdio>
+
+#include <cooperative_groups.h>
+
+#include "../../include/mcpm.h"
+#include "mcpm_device.cuh"
+
+namespace mcpm {
+namespace {
+
+constexpr int LG_CLUSTER = 8;        // CTAs that share a row
+constexpr int LG_THREADS = 512;
+constexpr int LG_SLICE = 16384;      // tokens whose counters a CTA holds at once (one word each)
+constexpr int LG_COUNT_BITS = 20;    // counter word: times in the history; above: last bias entry + 1
+constexpr int LG_MAX_HIST = (1 << LG_COUNT_BITS) - 1, LG_MAX_BIAS = (1 << (32 - LG_COUNT_BITS)) - 2;
+
+struct Best {
+    float v;
+    int t;
+};
+// Larger value first, then the lower token; a token above every other stands for "none".
+__device__ __forceinline__ void take(Best& a, const Best& b) {
+    if (b.v > a.v || (b.v == a.v && b.t < a.t)) a = b;
+}
+
+// A cluster of LG_CLUSTER CTAs per row, each with a contiguous share of the vocabulary.  The history
+// is counted into shared-memory words (integer atomics: the order does not matter), a bias entry
+// leaves its index there (the largest, hence the last entry, stays), and the logits stream past them.
+__global__ void __launch_bounds__(LG_THREADS) k_logits(const mcpm_logits_params p) {
+    extern __shared__ uint32_t words[];
+    __shared__ Best warp_best[LG_THREADS / 32], cta_best[LG_CLUSTER];
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    if (p.argmax) cluster.barrier_arrive();   // waited for before the first write to another CTA's memory
+    const int tid = threadIdx.x, rank = cluster.block_rank(), row = blockIdx.x / LG_CLUSTER;
+    const int share = ((p.n_vocab + LG_CLUSTER - 1) / LG_CLUSTER + 31) & ~31;   // whole mask words
+    const int lo = min(p.n_vocab, rank * share), hi = min(p.n_vocab, lo + share);
+    const float* x = p.logits + row * p.logits_stride;
+    float* out = p.out + row * p.out_stride;
+    const int* hist = p.hist ? p.hist + row * p.hist_stride : nullptr;
+    const int n_hist = hist ? (p.hist_len ? min(max(p.hist_len[row], 0), p.hist_max) : p.hist_max) : 0;
+    const int* bias_token = p.bias_token ? p.bias_token + row * p.bias_stride : nullptr;
+    const int n_bias = bias_token ? (p.bias_len ? min(max(p.bias_len[row], 0), p.bias_max) : p.bias_max) : 0;
+    const uint32_t* allow = p.allow ? p.allow + row * p.allow_stride : nullptr;
+    float rep = 1.0f, freq = 0.0f, pres = 0.0f;
+    if (n_hist) rep = p.penalties[3 * row], freq = p.penalties[3 * row + 1], pres = p.penalties[3 * row + 2];
+    Best best{-INFINITY, 0x7fffffff};
+    for (int s0 = lo; s0 < hi; s0 += LG_SLICE) {
+        const int n = min(LG_SLICE, hi - s0);
+        if (n_hist || n_bias) {
+            for (int i = tid; i < n; i += LG_THREADS) words[i] = 0u;
+            __syncthreads();
+            for (int i = tid; i < n_bias; i += LG_THREADS) {
+                const unsigned t = static_cast<unsigned>(bias_token[i]) - static_cast<unsigned>(s0);
+                if (t < static_cast<unsigned>(n)) atomicMax(&words[t], static_cast<uint32_t>(i + 1) << LG_COUNT_BITS);
+            }
+            __syncthreads();
+            for (int i = tid; i < n_hist; i += LG_THREADS) {
+                const unsigned t = static_cast<unsigned>(hist[i]) - static_cast<unsigned>(s0);
+                if (t < static_cast<unsigned>(n)) atomicAdd(&words[t], 1u);
+            }
+            __syncthreads();
+        }
+        for (int i = tid; i < n; i += LG_THREADS) {
+            const int t = s0 + i;
+            float v = x[t];
+            if (n_hist || n_bias) {
+                const uint32_t w = words[i];
+                const uint32_t c = w & LG_MAX_HIST, b = w >> LG_COUNT_BITS;
+                if (c) {
+                    v = v > 0.0f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
+                    v = __fsub_rn(v, __fadd_rn(__fmul_rn(freq, static_cast<float>(c)), pres));
+                }
+                if (b) v = __fadd_rn(v, p.bias[row * p.bias_stride + b - 1]);
+            }
+            if (allow && !(allow[t >> 5] >> (t & 31) & 1u)) v = -INFINITY;
+            out[t] = v;
+            if (v > best.v) best = Best{v, t};
+        }
+        __syncthreads();
+    }
+    if (!p.argmax) return;   // the whole grid
+    for (int o = 16; o >= 1; o >>= 1)
+        take(best, Best{__shfl_xor_sync(0xffffffffu, best.v, o), __shfl_xor_sync(0xffffffffu, best.t, o)});
+    if ((tid & 31) == 0) warp_best[tid >> 5] = best;
+    __syncthreads();
+    if (tid == 0) {
+        for (int w = 1; w < LG_THREADS / 32; ++w) take(best, warp_best[w]);
+    }
+    cluster.barrier_wait();   // every CTA of the row has started
+    if (tid == 0) {
+        *cluster.map_shared_rank(&cta_best[rank], 0) = best;
+    }
+    cluster.sync();
+    if (rank == 0 && tid == 0) {
+        for (int c = 1; c < LG_CLUSTER; ++c) take(best, cta_best[c]);
+        p.argmax[row] = best.t == 0x7fffffff ? -1 : best.t;
+    }
+}
+
+}  // namespace
+}  // namespace mcpm
+
+using namespace mcpm;
+
+extern "C" mcpm_status mcpm_logits_process(const mcpm_logits_params* params, void* stream) {
+    if (!params) return MCPM_BAD_ARG;
+    mcpm_logits_params p = *params;
+    if (p.logits_stride == 0) p.logits_stride = p.n_vocab;
+    if (p.out_stride == 0) p.out_stride = p.n_vocab;
+    if (p.hist_stride == 0) p.hist_stride = p.hist_max;
+    if (p.bias_stride == 0) p.bias_stride = p.bias_max;
+    const int mask_words = p.n_vocab > 0 ? (p.n_vocab - 1) / 32 + 1 : 0;
+    if (p.allow_stride == 0) p.allow_stride = mask_words;
+    if (p.n_seq <= 0 || p.n_vocab <= 0 || p.n_seq > (1 << 20) || p.n_vocab > (1 << 30) || !p.logits || !p.out ||
+        p.logits_stride < p.n_vocab || p.out_stride < p.n_vocab ||
+        (p.out == p.logits && p.out_stride != p.logits_stride))
+        return MCPM_BAD_ARG;
+    if (p.hist && (!p.penalties || p.hist_max < 0 || p.hist_max > LG_MAX_HIST || p.hist_stride < p.hist_max)) return MCPM_BAD_ARG;
+    if (p.bias_token && (!p.bias || p.bias_max < 0 || p.bias_max > LG_MAX_BIAS || p.bias_stride < p.bias_max)) return MCPM_BAD_ARG;
+    if (p.allow && p.allow_stride < mask_words) return MCPM_BAD_ARG;
+    cudaError_t e = cudaFuncSetAttribute(k_logits, cudaFuncAttributeMaxDynamicSharedMemorySize, LG_SLICE * 4);
+    if (e == cudaSuccess) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(static_cast<unsigned>(p.n_seq) * LG_CLUSTER);
+        cfg.blockDim = dim3(LG_THREADS);
+        cfg.dynamicSmemBytes = p.hist || p.bias_token ? LG_SLICE * 4 : 0;
+        cfg.stream = static_cast<cudaStream_t>(stream);
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = LG_CLUSTER;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        e = cudaLaunchKernelEx(&cfg, k_logits, p);
+    }
+    if (e == cudaSuccess) return MCPM_OK;
+    std::fprintf(stderr, "[mcpm] mcpm_logits_process: CUDA error: %s\n", cudaGetErrorString(e));
+    return MCPM_CUDA_ERROR;
+}

@@ -1,0 +1,72 @@
+// Geometry of a paged KV pool as the kernels of mcpm_paged.cu see it: which element row a
+// position of a sequence lies in, with page ids and positions from device memory that are
+// checked before anything is addressed through them.
+#pragma once
+#include <cstddef>
+#include <cstdint>
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+namespace mcpm {
+
+constexpr int PAGED_MAX_GROUP = 16;   // query heads per KV head
+
+// Unsigned division by a divisor fixed at launch (Granlund and Montgomery, "Division by invariant
+// integers using multiplication"): exact for numerators below 2^31, where the sum does not carry.
+struct FastDiv {
+    uint32_t mul, shift;
+    void set(uint32_t d) {
+        shift = 0;
+        while ((1ull << shift) < d) ++shift;
+        mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+    }
+    __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, mul) + n) >> shift; }
+};
+
+struct PagedGeom {
+    int n_head, n_head_kv, head_dim, page_size, n_pages, max_pages;
+    long long page_stride, row_stride, head_stride;   // elements
+    FastDiv by_page;
+
+    __device__ __forceinline__ int clamp_len(int n) const {   // max_pages * page_size <= 2^30 (host check)
+        return min(max(n, 0), max_pages * page_size);
+    }
+    // Page and slot of position j, 0 <= j < max_pages * page_size; false: the page is absent.
+    __device__ __forceinline__ bool locate(const int* __restrict__ table_row, int j, int& page, int& slot) const {
+        const int c = static_cast<int>(by_page.div(static_cast<uint32_t>(j)));
+        slot = j - c * page_size;
+        page = __ldg(table_row + c);
+        return static_cast<unsigned>(page) < static_cast<unsigned>(n_pages);
+    }
+    __device__ __forceinline__ long long row(int page, int slot, int head) const {
+        return page * page_stride + slot * row_stride + head * head_stride;
+    }
+    __device__ __forceinline__ size_t mass_at(int page, int slot, int head) const {   // [page][kv head][slot]
+        return (static_cast<size_t>(page) * n_head_kv + head) * page_size + slot;
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ float kv_load(T x);
+template <>
+__device__ __forceinline__ float kv_load(float x) { return x; }
+template <>
+__device__ __forceinline__ float kv_load(__half x) { return __half2float(x); }
+template <>
+__device__ __forceinline__ float kv_load(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+// Four values rounded to the cache type (nearest, ties to even: the engine's own rounding of an
+// fp16 cache) in one store.
+__device__ __forceinline__ void kv_store4(float* p, float4 x) { *reinterpret_cast<float4*>(p) = x; }
+__device__ __forceinline__ void kv_store4(__half* p, float4 x) {
+    __half2 h[2] = {__floats2half2_rn(x.x, x.y), __floats2half2_rn(x.z, x.w)};
+    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(h);
+}
+__device__ __forceinline__ void kv_store4(__nv_bfloat16* p, float4 x) {
+    __nv_bfloat162 h[2] = {__floats2bfloat162_rn(x.x, x.y), __floats2bfloat162_rn(x.z, x.w)};
+    *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(h);
+}
+
+}  // namespace mcpm

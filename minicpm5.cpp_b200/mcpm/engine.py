@@ -37,11 +37,33 @@ class mcpm_config(C.Structure):
                 ("sched", C.c_int), ("kv_type", C.c_int), ("reserved", C.c_int * 2)]
 
 
-KV_F32, KV_F16 = 0, 1
+KV_F32, KV_F16, KV_BF16 = 0, 1, 2   # KV_BF16: paged pools only
 GEMM_TCGEN05, GEMM_MMA = 0, 1
 
 
 P, I, F = C.c_void_p, C.c_int, C.c_float
+
+class mcpm_paged_config(C.Structure):
+    _fields_ = [("kv_type", I), ("n_head", I), ("n_head_kv", I), ("head_dim", I), ("page_size", I), ("n_pages", I),
+                ("max_seqs", I), ("max_pages", I), ("page_stride", C.c_int64), ("row_stride", C.c_int64),
+                ("head_stride", C.c_int64)]
+
+
+class mcpm_paged_pool(C.Structure):
+    _fields_ = [("k", P), ("v", P), ("mass", P)]
+
+
+class mcpm_paged_tokens(C.Structure):
+    _fields_ = [("n_tok", I), ("tok_seq", P), ("tok_slot", P), ("tok_pos", P), ("q", P), ("q_out", P),
+                ("q_stride", C.c_int64), ("k", P), ("v", P), ("kv_stride", C.c_int64), ("rope", P), ("rope_len", I)]
+
+
+class mcpm_logits_params(C.Structure):
+    _fields_ = [("n_seq", I), ("n_vocab", I), ("logits", P), ("out", P), ("logits_stride", C.c_int64),
+                ("out_stride", C.c_int64), ("hist", P), ("hist_len", P), ("hist_max", I), ("hist_stride", C.c_int64),
+                ("penalties", P), ("bias_token", P), ("bias", P), ("bias_len", P), ("bias_max", I),
+                ("bias_stride", C.c_int64), ("allow", P), ("allow_stride", C.c_int64), ("argmax", P)]
+
 
 # exported symbol -> (restype, argtypes); tests check that every declared symbol exists
 SIGNATURES = {
@@ -83,6 +105,15 @@ SIGNATURES = {
     "mcpm_gemv_q8k_timed": (I, [I, P, I, P, P, I, I, I, I, C.POINTER(F), P]),
     "mcpm_attention": (I, [P, P, P, P, P, I, I, P, P, P]),
     "mcpm_attention_noalloc": (I, [P, P, P, P, P, I, I, P, P, P]),
+    "mcpm_paged_workspace_bytes": (C.c_size_t, [C.POINTER(mcpm_paged_config)]),
+    "mcpm_rope_table": (I, [C.POINTER(F), I, I, F]),
+    "mcpm_paged_append": (I, [C.POINTER(mcpm_paged_config), C.POINTER(mcpm_paged_pool), P, I,
+                              C.POINTER(mcpm_paged_tokens), P]),
+    "mcpm_paged_attention": (I, [C.POINTER(mcpm_paged_config), C.POINTER(mcpm_paged_pool), P, P, I, P, C.c_int64, P, F,
+                                 P, C.c_size_t, P]),
+    "mcpm_paged_evict": (I, [C.POINTER(mcpm_paged_config), C.POINTER(mcpm_paged_pool), P, P, P, P, P, I, I, I, I, P,
+                             C.c_size_t, P]),
+    "mcpm_logits_process": (I, [C.POINTER(mcpm_logits_params), P]),
     "mcpm_trace_enable": (I, [P, I]),
     "mcpm_trace_read": (I, [P, C.POINTER(C.c_uint64), I]),
     "mcpm_tp_nccl_id": (I, [P]),
@@ -365,3 +396,72 @@ def sample_top_p_host(logits: np.ndarray, temperature: float, top_p: float, r: f
 def attention(q_ptr, k_ptr, v_ptr, kc_ptr, vc_ptr, pos, max_seq, out_ptr, out_q8k_ptr=None, stream=0) -> None:
     check(load_library().mcpm_attention(q_ptr, k_ptr, v_ptr, kc_ptr, vc_ptr, pos, max_seq, out_ptr, out_q8k_ptr,
                                         stream), "mcpm_attention")
+
+
+# ------------------------------------------------------------------ paged KV cache and logits (device pointers)
+def paged_config(kv_type: int, n_head: int, n_head_kv: int, head_dim: int, page_size: int, n_pages: int, max_seqs: int,
+                 max_pages: int, page_stride: int = 0, row_stride: int = 0, head_stride: int = 0) -> mcpm_paged_config:
+    """Geometry of a paged pool: strides in elements, all 0 for packed [page][slot][kv head][dim]."""
+    return mcpm_paged_config(kv_type, n_head, n_head_kv, head_dim, page_size, n_pages, max_seqs, max_pages, page_stride,
+                             row_stride, head_stride)
+
+
+def paged_pool(k_ptr: int, v_ptr: int, mass_ptr: int = 0) -> mcpm_paged_pool:
+    """One layer's pool; mass ([page][kv head][slot] floats) only where attention weights are accumulated."""
+    return mcpm_paged_pool(k_ptr, v_ptr, mass_ptr or None)
+
+
+def paged_workspace_bytes(cfg: mcpm_paged_config) -> int:
+    """Workspace of the calls with this configuration (zero-filled once by the caller); raises on an invalid one."""
+    n = load_library().mcpm_paged_workspace_bytes(C.byref(cfg))
+    if not n:
+        raise MCPMError(BAD_ARG, "mcpm_paged_workspace_bytes")
+    return n
+
+
+def rope_table(n_pos: int, head_dim: int = 128, rope_base: float = 5000000.0) -> np.ndarray:
+    """(cos, sin) of positions [0, n_pos), [n_pos][head_dim / 2][2] on the host."""
+    out = np.empty((n_pos, head_dim // 2, 2), np.float32)
+    check(load_library().mcpm_rope_table(_fptr(out), n_pos, head_dim, rope_base), "mcpm_rope_table")
+    return out
+
+
+def paged_append(cfg: mcpm_paged_config, pool: mcpm_paged_pool, table_ptr: int, n_tok: int, tok_slot: int, k_ptr: int,
+                 v_ptr: int, tok_seq: int = 0, tok_pos: int = 0, q: int = 0, q_out: int = 0, q_stride: int = 0,
+                 kv_stride: int = 0, rope: int = 0, rope_len: int = 0, n_seq: Optional[int] = None,
+                 stream: int = 0) -> None:
+    """Rotates q and k of n_tok tokens and writes k, v to slot tok_slot[i] of sequence tok_seq[i] (i if 0)."""
+    t = mcpm_paged_tokens(n_tok, tok_seq or None, tok_slot, tok_pos or None, q or None, q_out or None, q_stride, k_ptr,
+                          v_ptr, kv_stride, rope or None, rope_len)
+    check(load_library().mcpm_paged_append(cfg, pool, table_ptr, cfg.max_seqs if n_seq is None else n_seq, t, stream),
+          "mcpm_paged_append")
+
+
+def paged_attention(cfg: mcpm_paged_config, pool: mcpm_paged_pool, table_ptr: int, len_ptr: int, n_seq: int, q_ptr: int,
+                    out_ptr: int, ws_ptr: int, ws_bytes: int, q_stride: int = 0, scale: float = 0.0,
+                    stream: int = 0) -> None:
+    """One query per sequence over its pages; with pool.mass the weights are added to each position's mass."""
+    check(load_library().mcpm_paged_attention(cfg, pool, table_ptr, len_ptr, n_seq, q_ptr, q_stride, out_ptr, scale,
+                                              ws_ptr, ws_bytes, stream), "mcpm_paged_attention")
+
+
+def paged_evict(cfg: mcpm_paged_config, pool: mcpm_paged_pool, table_ptr: int, len_ptr: int, dst_table_ptr: int,
+                new_len_ptr: int, kept_ptr: int, n_seq: int, n_keep: int, n_sink: int, n_recent: int, ws_ptr: int,
+                ws_bytes: int, stream: int = 0) -> None:
+    """Copies the n_keep positions of largest mass (the first n_sink and last n_recent always) to dst_table's pages."""
+    check(load_library().mcpm_paged_evict(cfg, pool, table_ptr, len_ptr, dst_table_ptr, new_len_ptr, kept_ptr, n_seq,
+                                          n_keep, n_sink, n_recent, ws_ptr, ws_bytes, stream), "mcpm_paged_evict")
+
+
+def logits_process(logits_ptr: int, out_ptr: int, n_seq: int, n_vocab: int, hist: int = 0, hist_max: Optional[int] = None,
+                   hist_stride: int = 0, hist_len: int = 0, penalties: int = 0, bias_token: int = 0, bias: int = 0,
+                   bias_max: Optional[int] = None, bias_stride: int = 0, bias_len: int = 0, allow: int = 0,
+                   allow_stride: int = 0, argmax: int = 0, logits_stride: int = 0, out_stride: int = 0,
+                   stream: int = 0) -> None:
+    """Penalties, biases and a grammar mask on n_seq rows of logits, and their greedy tokens (see mcpm_logits_params).
+    hist_max / bias_max: entries of a row, the row stride if not given."""
+    p = mcpm_logits_params(n_seq, n_vocab, logits_ptr, out_ptr, logits_stride, out_stride, hist or None, hist_len or None,
+                           hist_stride if hist_max is None else hist_max, hist_stride, penalties or None,
+                           bias_token or None, bias or None, bias_len or None, bias_stride if bias_max is None else bias_max,
+                           bias_stride, allow or None, allow_stride, argmax or None)
+    check(load_library().mcpm_logits_process(p, stream), "mcpm_logits_process")
