@@ -51,79 +51,6 @@ __global__ void k_paged_append(const PagedGeom g, const AppendArgs a) {
     if (!is_v && x % per_head == 0 && a.mass) a.mass[g.mass_at(page, slot, head)] = 0.0f;
 }
 
-// ---------------------------------------------------------------- attention
-struct AttArgs {
-    const void *kc, *vc;
-    float* mass;
-    const int *table, *len;
-    const float* q;
-    long long q_stride;
-    float* out;
-    float scale;
-};
-
-constexpr int ATT_WARPS = 8;
-
-// One CTA per (sequence, KV head).  Per query head each warp takes every eighth position with a running
-// maximum m, sum l and weighted sum of V (D / 32 dims a lane); the warps are then joined.  The weights
-// of a head are final only then, so mass reads K a second time.
-template <typename T, int D>
-__global__ void k_paged_attention(const PagedGeom g, const AttArgs a) {
-    __shared__ float sm[ATT_WARPS], sl[ATT_WARPS], so[ATT_WARPS][D];
-    const int seq = blockIdx.x, kv = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int group = g.n_head / g.n_head_kv, n = g.clamp_len(a.len[seq]);
-    const int* row = a.table + static_cast<size_t>(seq) * g.max_pages;
-    const T *kc = static_cast<const T*>(a.kc), *vc = static_cast<const T*>(a.vc);
-    int page, slot;
-    for (int h = kv * group; h < (kv + 1) * group; ++h) {
-        const float* q = a.q + seq * a.q_stride + static_cast<size_t>(h) * D;
-        auto score = [&](long long at) {
-            float s = 0.0f;
-            for (int d = lane; d < D; d += 32) s = fmaf(q[d], kv_load(kc[at + d]), s);
-            for (int o = 16; o >= 1; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-            return s * a.scale;
-        };
-        float m = -INFINITY, l = 0.0f, o[D / 32] = {};
-        for (int j = warp; j < n; j += ATT_WARPS) {
-            if (!g.locate(row, j, page, slot)) continue;
-            const long long at = g.row(page, slot, kv);
-            const float s = score(at), top = fmaxf(m, s);
-            const float keep = m == -INFINITY ? 0.0f : expf(m - top), p = expf(s - top);
-            l = fmaf(l, keep, p);
-            for (int d = 0; d < D / 32; ++d) o[d] = fmaf(o[d], keep, p * kv_load(vc[at + lane + 32 * d]));
-            m = top;
-        }
-        if (lane == 0) sm[warp] = m, sl[warp] = l;
-        for (int d = 0; d < D / 32; ++d) so[warp][lane + 32 * d] = o[d];
-        __syncthreads();
-        float top = sm[0];
-        for (int w = 1; w < ATT_WARPS; ++w) top = fmaxf(top, sm[w]);
-        float sum = 0.0f, x = 0.0f;
-        for (int w = 0; w < ATT_WARPS; ++w) {
-            const float e = sm[w] == -INFINITY ? 0.0f : expf(sm[w] - top);
-            sum = fmaf(sl[w], e, sum);
-            if (tid < D) x = fmaf(so[w][tid], e, x);
-        }
-        if (tid < D) a.out[(static_cast<size_t>(seq) * g.n_head + h) * D + tid] = sum == 0.0f ? 0.0f : x / sum;
-        if (a.mass)
-            for (int j = warp; j < n; j += ATT_WARPS) {
-                if (!g.locate(row, j, page, slot)) continue;
-                const float s = score(g.row(page, slot, kv));
-                if (lane == 0) a.mass[g.mass_at(page, slot, kv)] += expf(s - top) / sum;
-            }
-        __syncthreads();
-    }
-}
-
-template <typename T>
-void launch_attention(const PagedGeom& g, const AttArgs& a, int n_seq, cudaStream_t s) {
-    const dim3 grid(n_seq, g.n_head_kv);
-    if (g.head_dim == 64)
-        k_paged_attention<T, 64><<<grid, 32 * ATT_WARPS, 0, s>>>(g, a);
-    else
-        k_paged_attention<T, 128><<<grid, 32 * ATT_WARPS, 0, s>>>(g, a);
-}
-
 // ---------------------------------------------------------------- eviction
 struct EvictArgs {
     void *kc, *vc;
@@ -278,12 +205,7 @@ mcpm_status check_pool(const mcpm_paged_pool* p) {
     return p && p->k && p->v && aligned16(p->k) && aligned16(p->v) ? MCPM_OK : MCPM_BAD_ARG;
 }
 
-size_t workspace_bytes(const PagedGeom& g) {
-    return sizeof(float) * static_cast<size_t>(g.n_pages) * g.page_size * g.n_head;
-}
-
-mcpm_status launched(const char* what) {
-    const cudaError_t e = cudaGetLastError();
+mcpm_status status(const char* what, cudaError_t e) {
     if (e == cudaSuccess) return MCPM_OK;
     std::fprintf(stderr, "[mcpm] %s: CUDA error: %s\n", what, cudaGetErrorString(e));
     return MCPM_CUDA_ERROR;
@@ -298,7 +220,7 @@ extern "C" {
 
 size_t mcpm_paged_workspace_bytes(const mcpm_paged_config* cfg) {
     PagedGeom g;
-    return geometry(cfg, g) == MCPM_OK ? workspace_bytes(g) : 0;
+    return geometry(cfg, g) == MCPM_OK ? paged_attention_workspace(g, cfg->max_seqs) : 0;
 }
 
 mcpm_status mcpm_rope_table(float* out, int n_pos, int head_dim, float rope_base) {
@@ -345,7 +267,7 @@ mcpm_status mcpm_paged_append(const mcpm_paged_config* cfg, const mcpm_paged_poo
         k_paged_append<__half><<<grid, 128, 0, s>>>(g, a);
     else
         k_paged_append<__nv_bfloat16><<<grid, 128, 0, s>>>(g, a);
-    return launched("mcpm_paged_append");
+    return status("mcpm_paged_append", cudaGetLastError());
 }
 
 mcpm_status mcpm_paged_attention(const mcpm_paged_config* cfg, const mcpm_paged_pool* pool, const int* table,
@@ -357,19 +279,13 @@ mcpm_status mcpm_paged_attention(const mcpm_paged_config* cfg, const mcpm_paged_
     if (st != MCPM_OK) return st;
     if (q_stride == 0) q_stride = static_cast<int64_t>(g.n_head) * g.head_dim;
     if (!table || !seq_len || !q || !out || !ws || n_seq <= 0 || n_seq > cfg->max_seqs || !aligned16(q) || !aligned16(out) ||
-        !aligned16(ws) || ws_bytes < workspace_bytes(g) || q_stride < static_cast<int64_t>(g.n_head) * g.head_dim ||
+        !aligned16(ws) || ws_bytes < paged_attention_workspace(g, cfg->max_seqs) || q_stride < static_cast<int64_t>(g.n_head) * g.head_dim ||
         q_stride % 4 || !(scale >= 0.0f))
         return MCPM_BAD_ARG;
-    AttArgs a{pool->k, pool->v, pool->mass, table, seq_len, q, q_stride, out,
-              scale == 0.0f ? 1.0f / sqrtf(static_cast<float>(g.head_dim)) : scale};
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (cfg->kv_type == MCPM_KV_F32)
-        launch_attention<float>(g, a, n_seq, s);
-    else if (cfg->kv_type == MCPM_KV_F16)
-        launch_attention<__half>(g, a, n_seq, s);
-    else
-        launch_attention<__nv_bfloat16>(g, a, n_seq, s);
-    return launched("mcpm_paged_attention");
+    if (scale == 0.0f) scale = 1.0f / sqrtf(static_cast<float>(g.head_dim));
+    return status("mcpm_paged_attention",
+                  launch_paged_attention(g, cfg->kv_type, cfg->max_seqs, pool->k, pool->v, pool->mass, table, seq_len, n_seq, q,
+                                         q_stride, out, scale, ws, static_cast<cudaStream_t>(stream)));
 }
 
 mcpm_status mcpm_paged_evict(const mcpm_paged_config* cfg, const mcpm_paged_pool* pool, const int* table,
@@ -381,7 +297,7 @@ mcpm_status mcpm_paged_evict(const mcpm_paged_config* cfg, const mcpm_paged_pool
     if (st != MCPM_OK) return st;
     if (!pool->mass || !table || !seq_len || !dst_table || dst_table == table || !new_len || !kept || !ws || n_seq <= 0 ||
         n_seq > cfg->max_seqs || n_keep <= 0 || n_sink < 0 || n_recent < 0 || n_sink > n_keep || n_recent > n_keep - n_sink ||
-        n_keep > g.max_pages * g.page_size || !aligned16(ws) || ws_bytes < workspace_bytes(g))
+        n_keep > g.max_pages * g.page_size || !aligned16(ws) || ws_bytes < paged_attention_workspace(g, cfg->max_seqs))
         return MCPM_BAD_ARG;
     EvictArgs a{pool->k, pool->v, pool->mass, table, seq_len, dst_table, new_len, kept, n_keep, n_sink, n_recent};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -393,7 +309,7 @@ mcpm_status mcpm_paged_evict(const mcpm_paged_config* cfg, const mcpm_paged_pool
         k_paged_evict_copy<__half><<<grid, 128, 0, s>>>(g, a);
     else
         k_paged_evict_copy<__nv_bfloat16><<<grid, 128, 0, s>>>(g, a);
-    return launched("mcpm_paged_evict");
+    return status("mcpm_paged_evict", cudaGetLastError());
 }
 
 }  // extern "C"

@@ -48,14 +48,12 @@ struct PagedGeom {
     }
 };
 
-template <typename T>
-__device__ __forceinline__ float kv_load(T x);
-template <>
-__device__ __forceinline__ float kv_load(float x) { return x; }
-template <>
-__device__ __forceinline__ float kv_load(__half x) { return __half2float(x); }
-template <>
-__device__ __forceinline__ float kv_load(__nv_bfloat16 x) { return __bfloat162float(x); }
+// Attention (mcpm_paged_attention.cu).
+constexpr int PAGED_MAX_CTAS = 320;   // most CTAs of a launch: sizes the workspace's partial results
+size_t paged_attention_workspace(const PagedGeom& g, int max_seqs);
+cudaError_t launch_paged_attention(const PagedGeom& g, int kv_type, int max_seqs, const void* kc, const void* vc, float* mass,
+                                   const int* table, const int* len, int n_seq, const float* q, long long q_stride, float* out,
+                                   float scale, void* ws, cudaStream_t s);
 
 // Four values rounded to the cache type (nearest, ties to even: the engine's own rounding of an
 // fp16 cache) in one store.

@@ -1,0 +1,632 @@
+// Attention of one query per sequence over a paged KV cache, in one pass over K and V:
+//   s_hj = scale q_h . K_j,  m_h = max_j s_hj,  l_h = sum_j exp(s_hj - m_h),
+//   out_h = sum_j exp(s_hj - m_h) V_j / l_h
+// with a running m, l and unnormalised output per warp, joined at the end of each (sequence, KV head).
+//
+// The g query heads of a KV head share its rows, so the products are matrix products with g columns:
+// S^T (16 positions x 8 heads) = K (16 x D) q^T and O^T (D x 8 heads) += V^T (D x 16) P^T, on warp-level
+// tensor-core instructions whose 8-wide N side the heads fill.  The work is bound by the bytes of K and V
+// (2 D esz per position and KV head against 4 g D operations), far below the rate at which 128-row
+// tensor-memory instructions would pay for their padding of g heads.
+//
+// fp32 results.  Operands of the cache type are exact; the fp32 operands (q, and the weights P) are split
+// into parts of that type, two for fp16 (22 bits), three for bf16 (24 bits); an fp32 cache is itself split
+// into two tf32 parts, with the three products that matter.  Accumulators are fp32.
+//
+// Work is split over the grid in units of 64 positions: the units of all (sequence, KV head) pairs in a
+// row, an equal share per CTA.  A pair that spans several CTAs leaves a partial result per CTA, and the
+// CTA that arrives last joins them in order of position, so results do not depend on arrival order.
+#include <algorithm>
+#include <cmath>
+
+#include "../../include/mcpm.h"
+#include "mcpm_device.cuh"
+#include "mcpm_paged.cuh"
+
+namespace mcpm {
+namespace {
+
+constexpr int WARPS = 4, THREADS = 32 * WARPS;
+constexpr int ROWS = 16;            // positions of a warp's tile
+constexpr int UNIT = ROWS * WARPS;  // positions of a unit of work
+constexpr int MIN_UNITS = 2;        // units that a CTA takes before the next CTA is used
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float P_SCALE = 1024.0f;  // weights are multiplied by this before they are split: fp16 parts of small
+                                    // weights stay normal; undone in the output
+
+template <typename T>
+constexpr int parts() { return sizeof(T) == 4 || __is_same(T, __half) ? 2 : 3; }
+
+template <typename T, int D, int NT>
+struct Tile {
+    static constexpr int RB = D * static_cast<int>(sizeof(T));
+    static constexpr int CHUNKS = RB / 16;
+    // Row pitches that make the fragment loads conflict-free: ldmatrix (8 rows of 16 bytes) wants 16 bytes
+    // more than a multiple of 128; the fp32 loads of 16 bytes per lane want, in words, 16 mod 32 for K (two
+    // rows of four lanes at a time) and 8 mod 32 for V (four rows of two lanes).
+    static constexpr int KP = sizeof(T) == 4 ? RB + 64 : RB + 16, VP = sizeof(T) == 4 ? RB + 32 : RB + 16;
+    static constexpr int HEAD = ROWS * 4;   // physical slot of each row, -1: not visible
+    static constexpr int STAGE = HEAD + ROWS * (KP + VP);
+    static constexpr int KSTEPS = sizeof(T) == 4 ? D / 8 : D / 16;
+    static constexpr int QWORDS = parts<T>() * 2;   // words of q per lane, k step and 8 heads
+    static constexpr int Q_BYTES = KSTEPS * NT * 32 * QWORDS * 4;
+    // Stages per warp: two CTAs per SM where three stages allow it, else one.
+    static constexpr int stages(int bytes) { return (bytes - Q_BYTES) / (WARPS * STAGE); }
+    static constexpr int CTAS = stages(112 * 1024) >= 3 ? 2 : 1;
+    static constexpr int STAGES = stages((CTAS == 2 ? 112 : 224) * 1024);
+    static constexpr int SMEM = WARPS * STAGES * STAGE + Q_BYTES;
+    static_assert(STAGES >= 2 && WARPS * 8 * NT * (D + 4) * 4 <= WARPS * STAGES * STAGE, "the rings hold the warps' outputs");
+};
+
+struct AttArgs {
+    const void *kc, *vc;
+    const int *table, *len;
+    const float* q;
+    long long q_stride;
+    float* out;
+    float scale;
+    int n_seq, group;
+    unsigned* cnt;     // [seq][kv head] arrivals, zero between calls
+    float2* stats;     // [seq][head] (max in units of log2, 1 / sum); mass only
+    float* part;       // [2 CTA + which][m[group], l[group], o[group][D]]
+    float* scores;     // [page * page_size + slot][n_head] scores in units of log2; mass only
+};
+
+__device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool fill) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(fill ? 0 : 16) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ float4 lds_f4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (sizeof(T) == 4)
+        asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else if constexpr (__is_same(T, __half))
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// x = hi + lo: hi the upper 11 significand bits, lo the rest rounded to 11 (the instruction drops the bits
+// below).  Truncating hi keeps finite values finite.
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+    hi = __float_as_uint(x) & 0xffffe000u;
+    lo = __float_as_uint(x - __uint_as_float(hi)) + 0x1000u;
+}
+// Part i of a value in 16-bit parts; x becomes what is left.
+template <typename T>
+__device__ __forceinline__ uint16_t take_part(float& x) {
+    if constexpr (__is_same(T, __half)) {
+        const __half h = __float2half_rn(x);
+        x -= __half2float(h);
+        return __half_as_ushort(h);
+    } else {
+        const __nv_bfloat16 h = __float2bfloat16_rn(x);
+        x -= __bfloat162float(h);
+        return __bfloat16_as_ushort(h);
+    }
+}
+template <typename T>
+__device__ __forceinline__ uint32_t take_parts2(float& x, float& y) {   // x in the lower half
+    const uint32_t a = take_part<T>(x);
+    return a | static_cast<uint32_t>(take_part<T>(y)) << 16;
+}
+
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
+
+// Where a flattened unit of work falls: CTA c of n takes units [c total / n, (c + 1) total / n).
+__device__ __forceinline__ long long share_start(long long total, int n, int c) { return total * c / n; }
+__device__ __forceinline__ int share_of(long long total, int n, long long unit) {
+    return static_cast<int>(((unit + 1) * n - 1) / total);
+}
+
+template <typename T, int D, int NT, bool MASS>
+__global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attention(const PagedGeom g, const AttArgs a) {
+    using L = Tile<T, D, NT>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ long long s_before[THREADS];
+    __shared__ long long s_base;
+    __shared__ int s_seq, s_last;
+    __shared__ float s_qf[8 * NT];              // scale of a head's scores in units of log2
+    __shared__ float s_m[WARPS][8 * NT], s_l[WARPS][8 * NT];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, t4 = lane & 3;
+    uint32_t* qs = reinterpret_cast<uint32_t*>(smem + WARPS * L::STAGES * L::STAGE);
+    uint8_t* ring = smem + warp * L::STAGES * L::STAGE;
+    float* comb = reinterpret_cast<float*>(smem);   // [warp][head][D + 4] once the rings are drained
+    const T *kc = static_cast<const T*>(a.kc), *vc = static_cast<const T*>(a.vc);
+    const int group = a.group, hkv = g.n_head_kv;
+
+    // ---- this CTA's share of the units
+    auto units_of = [&](int seq) { return (g.clamp_len(a.len[seq]) + UNIT - 1) / UNIT; };
+    const int per = (a.n_seq + THREADS - 1) / THREADS;
+    long long mine = 0;
+    for (int i = tid * per; i < min(a.n_seq, (tid + 1) * per); ++i) mine += units_of(i);
+    s_before[tid] = mine;
+    __syncthreads();
+    for (int o = 1; o < THREADS; o <<= 1) {   // inclusive scan
+        const long long x = tid >= o ? s_before[tid - o] : 0;
+        __syncthreads();
+        s_before[tid] += x;
+        __syncthreads();
+    }
+    const long long total = s_before[THREADS - 1] * hkv;
+    const int n_cta = static_cast<int>(min(static_cast<long long>(gridDim.x), (total + MIN_UNITS - 1) / MIN_UNITS));
+    // sequences without positions: zeros
+    for (int seq = blockIdx.x; seq < a.n_seq; seq += gridDim.x)
+        if (a.len[seq] <= 0)
+            for (int i = tid; i < g.n_head * D; i += THREADS) a.out[static_cast<size_t>(seq) * g.n_head * D + i] = 0.0f;
+    if (static_cast<int>(blockIdx.x) >= n_cta) return;
+    long long f = share_start(total, n_cta, blockIdx.x);
+    const long long f_end = share_start(total, n_cta, blockIdx.x + 1);
+    {
+        long long base = (s_before[tid] - mine) * hkv;
+        if (f >= base && f < base + mine * hkv)
+            for (int i = tid * per;; ++i) {
+                const long long n = static_cast<long long>(units_of(i)) * hkv;
+                if (f < base + n) {
+                    s_seq = i;
+                    s_base = base;
+                    break;
+                }
+                base += n;
+            }
+    }
+    __syncthreads();
+    int seq = s_seq;
+    long long seq_base = s_base;   // first unit of the sequence
+
+    while (f < f_end) {
+        const int units = units_of(seq);
+        if (f >= seq_base + static_cast<long long>(units) * hkv) {
+            seq_base += static_cast<long long>(units) * hkv;
+            ++seq;
+            continue;
+        }
+        const int kv = static_cast<int>((f - seq_base) / units);
+        const long long seg0 = seq_base + static_cast<long long>(kv) * units, seg1 = seg0 + units;
+        const int u0 = static_cast<int>(f - seg0), u1 = static_cast<int>(min(seg1, f_end) - seg0);
+        f = min(seg1, f_end);
+        const int len = g.clamp_len(a.len[seq]);
+        const int* row = a.table + static_cast<size_t>(seq) * g.max_pages;
+
+        // ---- copies of K and V rows: lane & 15 looks a row of the tile up, all lanes copy
+        auto lookup = [&](int tile, int& page) {   // tile: this warp's tiles u0 .. u1 - 1
+            const int j = tile * UNIT + warp * ROWS + (lane & 15);
+            page = -1;
+            if (tile < u1 && j < len) page = __ldg(row + g.by_page.div(static_cast<uint32_t>(j)));
+        };
+        auto issue = [&](int tile, int page) {
+            if (tile < u1) {
+                uint8_t* st = ring + (tile - u0) % L::STAGES * L::STAGE;
+                const int j = tile * UNIT + warp * ROWS + (lane & 15);
+                const int slot = j - static_cast<int>(g.by_page.div(static_cast<uint32_t>(j))) * g.page_size;
+                const bool ok = static_cast<unsigned>(page) < static_cast<unsigned>(g.n_pages);
+                const long long off = ok ? g.row(page, slot, kv) : -1;
+                if (lane < 16) reinterpret_cast<int*>(st)[lane] = ok ? page * g.page_size + slot : -1;
+                const uint32_t kd = smem_u32(st + L::HEAD), vd = kd + ROWS * L::KP;
+#pragma unroll
+                for (int i = 0; i < ROWS * L::CHUNKS / 32; ++i) {
+                    const int r = i * (32 / L::CHUNKS) + lane / L::CHUNKS, c = lane % L::CHUNKS;
+                    const long long o = __shfl_sync(0xffffffffu, off, r);
+                    const size_t at = (o < 0 ? 0 : o) + c * (16 / sizeof(T));
+                    cp_async16_zfill(kd + r * L::KP + c * 16, kc + at, o < 0);
+                    cp_async16_zfill(vd + r * L::VP + c * 16, vc + at, o < 0);
+                }
+            }
+            cp_async_commit();
+        };
+        int next_page;
+#pragma unroll 1
+        for (int i = 0; i < L::STAGES - 1; ++i) {
+            int page;
+            lookup(u0 + i, page);
+            issue(u0 + i, page);
+        }
+        lookup(u0 + L::STAGES - 1, next_page);
+
+        // ---- q in fragment order, normalised per head to [2^7, 2^8) so that 16-bit parts neither overflow
+        // nor vanish
+        for (int h = warp; h < 8 * NT; h += WARPS) {
+            float x[D / 32];
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i)
+                x[i] = h < group ? a.q[seq * a.q_stride + static_cast<size_t>(kv * group + h) * D + lane + 32 * i] : 0.0f;
+            float top = 0.0f;
+            for (int i = 0; i < D / 32; ++i) top = fmaxf(top, fabsf(x[i]));
+            for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            const int e = min(max(7 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), -120), 120);
+            const float up = pow2(e);
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) {
+                float v = x[i] * up;
+                const int d = lane + 32 * i;
+                if constexpr (sizeof(T) == 4) {
+                    // dims 16 c + 4 t + (0, 1, 2, 3) of lane t: k = t and t + 4 of steps 2c and 2c + 1
+                    const int ks = 2 * (d / 16) + ((d >> 1) & 1), t = (d >> 2) & 3, w = d & 1;
+                    uint32_t* p = qs + ((ks * NT + (h >> 3)) * 32 + (h & 7) * 4 + t) * 4;
+                    uint32_t hi, lo;
+                    split_tf32(v, hi, lo);
+                    p[w] = hi;
+                    p[2 + w] = lo;
+                } else {
+                    const int ks = d / 16, r = d & 15, t = (r & 7) >> 1, w = r >> 3;
+                    uint16_t* p = reinterpret_cast<uint16_t*>(qs + ((ks * NT + (h >> 3)) * 32 + (h & 7) * 4 + t) * L::QWORDS + w) + (r & 1);
+#pragma unroll
+                    for (int k = 0; k < parts<T>(); ++k) p[4 * k] = take_part<T>(v);
+                }
+            }
+            if (lane == 0) s_qf[h] = a.scale * LOG2E * pow2(-e);
+        }
+        __syncthreads();
+        float qf[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) qf[nt][0] = s_qf[8 * nt + 2 * t4], qf[nt][1] = s_qf[8 * nt + 2 * t4 + 1];
+
+        float o[NT][D / 16][4], m[NT][2], l[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            m[nt][0] = m[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.0f;
+        }
+
+        for (int tile = u0; tile < u1; ++tile) {
+            cp_async_wait_group<L::STAGES - 2>();
+            __syncwarp();   // the tile is in shared memory for all lanes, and all are done with the slot that follows
+            issue(tile + L::STAGES - 1, next_page);
+            lookup(tile + L::STAGES, next_page);
+            const uint8_t* st = ring + (tile - u0) % L::STAGES * L::STAGE;
+            const int where0 = reinterpret_cast<const int*>(st)[gq], where1 = reinterpret_cast<const int*>(st)[gq + 8];
+            const uint32_t ks = smem_u32(st + L::HEAD), vs = ks + ROWS * L::KP;
+
+            // ---- scores
+            float s[NT][4], s_lo[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[nt][i] = s_lo[nt][i] = 0.0f;
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int c = 0; c < D / 16; ++c) {
+                    const float4 r0 = lds_f4(ks + gq * L::KP + (16 * c + 4 * t4) * 4);
+                    const float4 r8 = lds_f4(ks + (gq + 8) * L::KP + (16 * c + 4 * t4) * 4);
+                    uint32_t hi[2][4], lo[2][4];
+                    split_tf32(r0.x, hi[0][0], lo[0][0]);
+                    split_tf32(r8.x, hi[0][1], lo[0][1]);
+                    split_tf32(r0.y, hi[0][2], lo[0][2]);
+                    split_tf32(r8.y, hi[0][3], lo[0][3]);
+                    split_tf32(r0.z, hi[1][0], lo[1][0]);
+                    split_tf32(r8.z, hi[1][1], lo[1][1]);
+                    split_tf32(r0.w, hi[1][2], lo[1][2]);
+                    split_tf32(r8.w, hi[1][3], lo[1][3]);
+#pragma unroll
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            const uint4 b = *reinterpret_cast<const uint4*>(qs + (((2 * c + k) * NT + nt) * 32 + lane) * 4);
+                            mma<T>(s[nt], hi[k], b.x, b.y);
+                            mma<T>(s_lo[nt], hi[k], b.z, b.w);
+                            mma<T>(s_lo[nt], lo[k], b.x, b.y);
+                        }
+                }
+            } else {
+#pragma unroll
+                for (int c = 0; c < D / 16; ++c) {
+                    uint32_t k[4];
+                    ldsm4(k, ks + ((lane & 7) + (lane & 8)) * L::KP + (16 * c + (lane >> 4) * 8) * 2);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const uint2* b = reinterpret_cast<const uint2*>(qs + ((c * NT + nt) * 32 + lane) * L::QWORDS);
+                        mma<T>(s[nt], k, b[0].x, b[0].y);
+#pragma unroll
+                        for (int p = 1; p < parts<T>(); ++p) mma<T>(s_lo[nt], k, b[p].x, b[p].y);
+                    }
+                }
+            }
+            // ---- weights: lane (gq, t4) holds positions gq, gq + 8 of heads 2 t4, 2 t4 + 1
+            bool grown = false;
+            float top[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[nt][i] += s_lo[nt][i];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float x = where0 >= 0 ? s[nt][i] * qf[nt][i] : -INFINITY;
+                    const float y = where1 >= 0 ? s[nt][2 + i] * qf[nt][i] : -INFINITY;
+                    if constexpr (MASS) {
+                        const int h = 8 * nt + 2 * t4 + i;
+                        if (h < group && where0 >= 0) a.scores[static_cast<size_t>(where0) * g.n_head + kv * group + h] = x;
+                        if (h < group && where1 >= 0) a.scores[static_cast<size_t>(where1) * g.n_head + kv * group + h] = y;
+                    }
+                    float v = fmaxf(x, y);
+                    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+                    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+                    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+                    top[nt][i] = fmaxf(m[nt][i], v);
+                    grown |= v > m[nt][i];
+                }
+            }
+            if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    float keep[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        keep[i] = m[nt][i] == -INFINITY ? 0.0f : exp2f(m[nt][i] - top[nt][i]);
+                        l[nt][i] *= keep[i];
+                        m[nt][i] = top[nt][i];
+                    }
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        o[nt][i][0] *= keep[0];
+                        o[nt][i][1] *= keep[1];
+                        o[nt][i][2] *= keep[0];
+                        o[nt][i][3] *= keep[1];
+                    }
+                }
+            }
+            float p[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float ref = m[nt][i] == -INFINITY ? 0.0f : m[nt][i];
+                    p[nt][i] = where0 >= 0 ? exp2f(__fmaf_rn(s[nt][i], qf[nt][i], -ref)) : 0.0f;
+                    p[nt][2 + i] = where1 >= 0 ? exp2f(__fmaf_rn(s[nt][2 + i], qf[nt][i], -ref)) : 0.0f;
+                    l[nt][i] += p[nt][i] + p[nt][2 + i];
+                    p[nt][i] *= P_SCALE;
+                    p[nt][2 + i] *= P_SCALE;
+                }
+            // ---- O^T += V^T P^T
+            if constexpr (sizeof(T) == 4) {
+                uint32_t ph[NT][2][2], pl[NT][2][2];   // [8 positions][k = t4, t4 + 4]
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+                        for (int w = 0; w < 2; ++w) {
+                            const int src = 4 * (t4 + 4 * w) + (gq >> 1);
+                            const float x = __shfl_sync(0xffffffffu, p[nt][2 * kk], src);
+                            const float y = __shfl_sync(0xffffffffu, p[nt][2 * kk + 1], src);
+                            split_tf32(gq & 1 ? y : x, ph[nt][kk][w], pl[nt][kk][w]);
+                        }
+#pragma unroll
+                for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+                    for (int kk = 0; kk < 2; ++kk) {
+                        const float4 r0 = lds_f4(vs + (8 * kk + t4) * L::VP + (32 * b + 4 * gq) * 4);
+                        const float4 r4 = lds_f4(vs + (8 * kk + t4 + 4) * L::VP + (32 * b + 4 * gq) * 4);
+                        uint32_t hi[2][4], lo[2][4];
+                        split_tf32(r0.x, hi[0][0], lo[0][0]);
+                        split_tf32(r0.y, hi[0][1], lo[0][1]);
+                        split_tf32(r4.x, hi[0][2], lo[0][2]);
+                        split_tf32(r4.y, hi[0][3], lo[0][3]);
+                        split_tf32(r0.z, hi[1][0], lo[1][0]);
+                        split_tf32(r0.w, hi[1][1], lo[1][1]);
+                        split_tf32(r4.z, hi[1][2], lo[1][2]);
+                        split_tf32(r4.w, hi[1][3], lo[1][3]);
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                mma<T>(o[nt][2 * b + i], hi[i], ph[nt][kk][0], ph[nt][kk][1]);
+                                mma<T>(o[nt][2 * b + i], hi[i], pl[nt][kk][0], pl[nt][kk][1]);
+                                mma<T>(o[nt][2 * b + i], lo[i], ph[nt][kk][0], ph[nt][kk][1]);
+                            }
+                    }
+            } else {
+                uint32_t pb[NT][parts<T>()][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int k = 0; k < parts<T>(); ++k) {
+                        pb[nt][k][0] = transpose8x8(take_parts2<T>(p[nt][0], p[nt][1]));
+                        pb[nt][k][1] = transpose8x8(take_parts2<T>(p[nt][2], p[nt][3]));
+                    }
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    uint32_t v[4];
+                    ldsm4_t(v, vs + ((lane & 7) + (lane >> 4) * 8) * L::VP + (16 * i + (lane & 8)) * 2);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int k = 0; k < parts<T>(); ++k) mma<T>(o[nt][i], v, pb[nt][k][0], pb[nt][k][1]);
+                }
+            }
+        }
+        cp_async_wait_all();
+
+        // ---- the CTA's result for this (sequence, KV head)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float x = l[nt][i];
+                x += __shfl_xor_sync(0xffffffffu, x, 4);
+                x += __shfl_xor_sync(0xffffffffu, x, 8);
+                x += __shfl_xor_sync(0xffffffffu, x, 16);
+                if (gq == 0) s_m[warp][8 * nt + 2 * t4 + i] = m[nt][i], s_l[warp][8 * nt + 2 * t4 + i] = x;
+            }
+        __syncthreads();   // rings are drained: their memory holds the warps' outputs now
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int d = sizeof(T) == 4 ? 32 * (i / 2) + 4 * gq + 2 * (i & 1) + (e >> 1) : 16 * i + gq + 8 * (e >> 1);
+                    comb[((warp * NT + nt) * 8 + 2 * t4 + (e & 1)) * (D + 4) + d] = o[nt][i][e];
+                }
+        __syncthreads();
+        const int first = share_of(total, n_cta, seg0), last = share_of(total, n_cta, seg1 - 1);
+        const int rec = group * (2 + D);   // floats of a partial result
+        float* part = a.part + (2 * static_cast<size_t>(blockIdx.x) + (static_cast<int>(blockIdx.x) == first)) * rec;
+        float* out = a.out + (static_cast<size_t>(seq) * g.n_head + kv * group) * D;
+        float2* stats = a.stats + static_cast<size_t>(seq) * g.n_head + kv * group;
+        for (int i = tid; i < group * D; i += THREADS) {
+            const int h = i / D, d = i % D;
+            float top = s_m[0][h];
+#pragma unroll
+            for (int w = 1; w < WARPS; ++w) top = fmaxf(top, s_m[w][h]);
+            float sum = 0.0f, x = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                const float e = s_m[w][h] == -INFINITY ? 0.0f : exp2f(s_m[w][h] - top);
+                sum = fmaf(s_l[w][h], e, sum);
+                x = fmaf(comb[((w * NT + (h >> 3)) * 8 + (h & 7)) * (D + 4) + d], e, x);
+            }
+            if (first == last) {
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                out[i] = x * (1.0f / P_SCALE) * inv;
+                if (MASS && d == 0) stats[h] = make_float2(top, inv);
+            } else {
+                part[2 * group + i] = x;
+                if (d == 0) part[h] = top, part[group + h] = sum;
+            }
+        }
+        if (first != last) {
+            __threadfence();
+            __syncthreads();
+            if (tid == 0) {
+                unsigned* c = a.cnt + seq * hkv + kv;
+                s_last = atomicAdd(c, 1u) == static_cast<unsigned>(last - first);
+                if (s_last) *c = 0u;
+            }
+            __syncthreads();
+            if (s_last) {
+                __threadfence();
+                const int np = last - first + 1;
+                auto record = [&](int k) { return a.part + (2 * static_cast<size_t>(first + k) + (k == 0)) * rec; };
+                for (int i = tid; i < group * D; i += THREADS) {
+                    const int h = i / D, d = i % D;
+                    float top = -INFINITY, sum = 0.0f, x = 0.0f;
+                    for (int k = 0; k < np; ++k) top = fmaxf(top, __ldcg(record(k) + h));
+                    for (int k = 0; k < np; ++k) {
+                        const float* r = record(k);
+                        const float mk = __ldcg(r + h);
+                        const float e = mk == -INFINITY ? 0.0f : exp2f(mk - top);
+                        sum = fmaf(__ldcg(r + group + h), e, sum);
+                        x = fmaf(__ldcg(r + 2 * group + i), e, x);
+                    }
+                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                    out[i] = x * (1.0f / P_SCALE) * inv;
+                    if (MASS && d == 0) stats[h] = make_float2(top, inv);
+                }
+            }
+        }
+        __syncthreads();   // comb and s_m are free for the next pair
+    }
+}
+
+// mass[position] += sum over the KV head's query heads of exp(s - max) / sum.  A thread per (position,
+// KV head); grid.y sequences, grid.x equal shares of a sequence.
+__global__ void k_paged_mass(const PagedGeom g, const AttArgs a, float* __restrict__ mass) {
+    extern __shared__ float2 st[];
+    grid_dep_wait();
+    const int seq = blockIdx.y, n = g.clamp_len(a.len[seq]), hkv = g.n_head_kv;
+    for (int i = threadIdx.x; i < g.n_head; i += blockDim.x) st[i] = a.stats[static_cast<size_t>(seq) * g.n_head + i];
+    __syncthreads();
+    const int* row = a.table + static_cast<size_t>(seq) * g.max_pages;
+    const long long items = static_cast<long long>(n) * hkv;
+    for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < items; i += static_cast<long long>(gridDim.x) * blockDim.x) {
+        const int j = static_cast<int>(i / hkv), kv = static_cast<int>(i % hkv);
+        int page, slot;
+        if (!g.locate(row, j, page, slot)) continue;
+        const float* s = a.scores + (static_cast<size_t>(page) * g.page_size + slot) * g.n_head + kv * a.group;
+        float w = 0.0f;
+        for (int h = 0; h < a.group; ++h) w = fmaf(exp2f(s[h] - st[kv * a.group + h].x), st[kv * a.group + h].y, w);
+        mass[g.mass_at(page, slot, kv)] += w;
+    }
+}
+
+constexpr size_t up(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
+size_t part_floats(const PagedGeom& g) {
+    return 2ull * PAGED_MAX_CTAS * (g.n_head / g.n_head_kv) * (2 + g.head_dim);
+}
+
+template <typename T, int D, int NT, bool MASS>
+cudaError_t run(const PagedGeom& g, const AttArgs& a, float* mass, int n_sm, cudaStream_t s) {
+    using L = Tile<T, D, NT>;
+    auto* kernel = k_paged_attention<T, D, NT, MASS>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+    if (e != cudaSuccess) return e;
+    const int grid = std::min(n_sm * L::CTAS, PAGED_MAX_CTAS);
+    kernel<<<grid, THREADS, L::SMEM, s>>>(g, a);
+    e = cudaGetLastError();
+    if (e != cudaSuccess || !MASS) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(std::max(1, (4 * n_sm + a.n_seq - 1) / a.n_seq), a.n_seq);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = g.n_head * sizeof(float2);
+    cfg.stream = s;
+    return cudaLaunchKernelEx(&cfg, k_paged_mass, g, a, mass);
+}
+
+template <typename T>
+cudaError_t pick(const PagedGeom& g, const AttArgs& a, float* mass, int n_sm, cudaStream_t s) {
+    const bool two = a.group > 8;   // heads beside the 8 of one instruction
+    if (g.head_dim == 64)
+        return mass ? (two ? run<T, 64, 2, true>(g, a, mass, n_sm, s) : run<T, 64, 1, true>(g, a, mass, n_sm, s))
+                    : (two ? run<T, 64, 2, false>(g, a, mass, n_sm, s) : run<T, 64, 1, false>(g, a, mass, n_sm, s));
+    return mass ? (two ? run<T, 128, 2, true>(g, a, mass, n_sm, s) : run<T, 128, 1, true>(g, a, mass, n_sm, s))
+                : (two ? run<T, 128, 2, false>(g, a, mass, n_sm, s) : run<T, 128, 1, false>(g, a, mass, n_sm, s));
+}
+
+}  // namespace
+
+size_t paged_attention_workspace(const PagedGeom& g, int max_seqs) {
+    return up(sizeof(unsigned) * max_seqs * g.n_head_kv) + up(sizeof(float2) * max_seqs * g.n_head) +
+           up(sizeof(float) * part_floats(g)) + sizeof(float) * static_cast<size_t>(g.n_pages) * g.page_size * g.n_head;
+}
+
+cudaError_t launch_paged_attention(const PagedGeom& g, int kv_type, int max_seqs, const void* kc, const void* vc, float* mass,
+                                   const int* table, const int* len, int n_seq, const float* q, long long q_stride, float* out,
+                                   float scale, void* ws, cudaStream_t s) {
+    static int n_sms[64] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!n_sms[dev]) {
+        int n = 0;
+        e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+        if (e != cudaSuccess) return e;
+        n_sms[dev] = n;
+    }
+    uint8_t* w = static_cast<uint8_t*>(ws);
+    AttArgs a{kc, vc, table, len, q, q_stride, out, scale, n_seq, g.n_head / g.n_head_kv};
+    a.cnt = reinterpret_cast<unsigned*>(w);
+    w += up(sizeof(unsigned) * max_seqs * g.n_head_kv);
+    a.stats = reinterpret_cast<float2*>(w);
+    w += up(sizeof(float2) * max_seqs * g.n_head);
+    a.part = reinterpret_cast<float*>(w);
+    w += up(sizeof(float) * part_floats(g));
+    a.scores = reinterpret_cast<float*>(w);
+    if (kv_type == MCPM_KV_F32) return pick<float>(g, a, mass, n_sms[dev], s);
+    if (kv_type == MCPM_KV_F16) return pick<__half>(g, a, mass, n_sms[dev], s);
+    return pick<__nv_bfloat16>(g, a, mass, n_sms[dev], s);
+}
+
+}  // namespace mcpm
