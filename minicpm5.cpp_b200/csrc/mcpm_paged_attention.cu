@@ -68,7 +68,7 @@ struct AttArgs {
     int n_seq, group;
     unsigned* cnt;     // [seq][kv head] arrivals, zero between calls
     float2* stats;     // [seq][head] (max in units of log2, 1 / sum); mass only
-    float* part;       // [2 CTA + which][m[group], l[group], o[group][D]]
+    float* part;       // [2 CTA + which][m[group], l[group], pad to 32, o[group][D]]
     float* scores;     // [page * page_size + slot][n_head] scores in units of log2; mass only
 };
 
@@ -143,8 +143,7 @@ template <typename T, int D, int NT, bool MASS>
 __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attention(const PagedGeom g, const AttArgs a) {
     using L = Tile<T, D, NT>;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ long long s_before[THREADS];
-    __shared__ long long s_base;
+    __shared__ long long s_sum[WARPS], s_base;
     __shared__ int s_seq, s_last;
     __shared__ float s_qf[8 * NT];              // scale of a head's scores in units of log2
     __shared__ float s_m[WARPS][8 * NT], s_l[WARPS][8 * NT];
@@ -160,15 +159,21 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
     const int per = (a.n_seq + THREADS - 1) / THREADS;
     long long mine = 0;
     for (int i = tid * per; i < min(a.n_seq, (tid + 1) * per); ++i) mine += units_of(i);
-    s_before[tid] = mine;
-    __syncthreads();
-    for (int o = 1; o < THREADS; o <<= 1) {   // inclusive scan
-        const long long x = tid >= o ? s_before[tid - o] : 0;
-        __syncthreads();
-        s_before[tid] += x;
-        __syncthreads();
+    long long before = mine;   // inclusive scan over the threads
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += x;
     }
-    const long long total = s_before[THREADS - 1] * hkv;
+    if (lane == 31) s_sum[warp] = before;
+    __syncthreads();
+    long long total = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+        if (w < warp) before += s_sum[w];
+        total += s_sum[w];
+    }
+    before = (before - mine) * hkv;
+    total *= hkv;
     const int n_cta = static_cast<int>(min(static_cast<long long>(gridDim.x), (total + MIN_UNITS - 1) / MIN_UNITS));
     // sequences without positions: zeros
     for (int seq = blockIdx.x; seq < a.n_seq; seq += gridDim.x)
@@ -178,7 +183,7 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
     long long f = share_start(total, n_cta, blockIdx.x);
     const long long f_end = share_start(total, n_cta, blockIdx.x + 1);
     {
-        long long base = (s_before[tid] - mine) * hkv;
+        long long base = before;
         if (f >= base && f < base + mine * hkv)
             for (int i = tid * per;; ++i) {
                 const long long n = static_cast<long long>(units_of(i)) * hkv;
@@ -300,11 +305,12 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
             const uint32_t ks = smem_u32(st + L::HEAD), vs = ks + ROWS * L::KP;
 
             // ---- scores
-            float s[NT][4], s_lo[NT][4];
+            // Independent accumulators: the instruction truncates, so short chains lose less, and they overlap.
+            float s[NT][4], s_hi[NT][2][4], s_lo[NT][4];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[nt][i] = s_lo[nt][i] = 0.0f;
+                for (int i = 0; i < 4; ++i) s_hi[nt][0][i] = s_hi[nt][1][i] = s_lo[nt][i] = 0.0f;
             if constexpr (sizeof(T) == 4) {
 #pragma unroll
                 for (int c = 0; c < D / 16; ++c) {
@@ -324,7 +330,7 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
                             const uint4 b = *reinterpret_cast<const uint4*>(qs + (((2 * c + k) * NT + nt) * 32 + lane) * 4);
-                            mma<T>(s[nt], hi[k], b.x, b.y);
+                            mma<T>(s_hi[nt][k], hi[k], b.x, b.y);
                             mma<T>(s_lo[nt], hi[k], b.z, b.w);
                             mma<T>(s_lo[nt], lo[k], b.x, b.y);
                         }
@@ -337,19 +343,18 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         const uint2* b = reinterpret_cast<const uint2*>(qs + ((c * NT + nt) * 32 + lane) * L::QWORDS);
-                        mma<T>(s[nt], k, b[0].x, b[0].y);
+                        mma<T>(s_hi[nt][c & 1], k, b[0].x, b[0].y);
 #pragma unroll
                         for (int p = 1; p < parts<T>(); ++p) mma<T>(s_lo[nt], k, b[p].x, b[p].y);
                     }
                 }
             }
             // ---- weights: lane (gq, t4) holds positions gq, gq + 8 of heads 2 t4, 2 t4 + 1
-            bool grown = false;
-            float top[NT][2];
+            float keep[NT][2];   // factor of what was summed before this tile
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[nt][i] += s_lo[nt][i];
+                for (int i = 0; i < 4; ++i) s[nt][i] = s_hi[nt][0][i] + s_hi[nt][1][i] + s_lo[nt][i];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const float x = where0 >= 0 ? s[nt][i] * qf[nt][i] : -INFINITY;
@@ -363,27 +368,10 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
                     v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
                     v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
                     v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-                    top[nt][i] = fmaxf(m[nt][i], v);
-                    grown |= v > m[nt][i];
-                }
-            }
-            if (__any_sync(0xffffffffu, grown)) {
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    float keep[2];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        keep[i] = m[nt][i] == -INFINITY ? 0.0f : exp2f(m[nt][i] - top[nt][i]);
-                        l[nt][i] *= keep[i];
-                        m[nt][i] = top[nt][i];
-                    }
-#pragma unroll
-                    for (int i = 0; i < D / 16; ++i) {
-                        o[nt][i][0] *= keep[0];
-                        o[nt][i][1] *= keep[1];
-                        o[nt][i][2] *= keep[0];
-                        o[nt][i][3] *= keep[1];
-                    }
+                    const float top = fmaxf(m[nt][i], v);
+                    keep[nt][i] = m[nt][i] == -INFINITY ? 0.0f : exp2f(m[nt][i] - top);
+                    l[nt][i] *= keep[nt][i];
+                    m[nt][i] = top;
                 }
             }
             float p[NT][4];
@@ -398,7 +386,12 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
                     p[nt][i] *= P_SCALE;
                     p[nt][2 + i] *= P_SCALE;
                 }
-            // ---- O^T += V^T P^T
+            // ---- O^T += V^T P^T, the tile's product from zero and then added: the instruction truncates its sums
+            // (one accumulator over 131072 positions lost three times the error of everything else)
+            auto add = [&](int nt, int i, const float (&x)[4]) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[nt][i][e] = fmaf(o[nt][i][e], keep[nt][e & 1], x[e]);
+            };
             if constexpr (sizeof(T) == 4) {
                 uint32_t ph[NT][2][2], pl[NT][2][2];   // [8 positions][k = t4, t4 + 4]
 #pragma unroll
@@ -414,6 +407,8 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
                         }
 #pragma unroll
                 for (int b = 0; b < D / 32; ++b)
+                {
+                    float x[2][NT][4] = {};
 #pragma unroll
                     for (int kk = 0; kk < 2; ++kk) {
                         const float4 r0 = lds_f4(vs + (8 * kk + t4) * L::VP + (32 * b + 4 * gq) * 4);
@@ -431,11 +426,16 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
                         for (int i = 0; i < 2; ++i)
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt) {
-                                mma<T>(o[nt][2 * b + i], hi[i], ph[nt][kk][0], ph[nt][kk][1]);
-                                mma<T>(o[nt][2 * b + i], hi[i], pl[nt][kk][0], pl[nt][kk][1]);
-                                mma<T>(o[nt][2 * b + i], lo[i], ph[nt][kk][0], ph[nt][kk][1]);
+                                mma<T>(x[i][nt], hi[i], ph[nt][kk][0], ph[nt][kk][1]);
+                                mma<T>(x[i][nt], hi[i], pl[nt][kk][0], pl[nt][kk][1]);
+                                mma<T>(x[i][nt], lo[i], ph[nt][kk][0], ph[nt][kk][1]);
                             }
                     }
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) add(nt, 2 * b + i, x[i][nt]);
+                }
             } else {
                 uint32_t pb[NT][parts<T>()][2];
 #pragma unroll
@@ -450,9 +450,12 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
                     uint32_t v[4];
                     ldsm4_t(v, vs + ((lane & 7) + (lane >> 4) * 8) * L::VP + (16 * i + (lane & 8)) * 2);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float x[4] = {};
 #pragma unroll
-                        for (int k = 0; k < parts<T>(); ++k) mma<T>(o[nt][i], v, pb[nt][k][0], pb[nt][k][1]);
+                        for (int k = 0; k < parts<T>(); ++k) mma<T>(x, v, pb[nt][k][0], pb[nt][k][1]);
+                        add(nt, i, x);
+                    }
                 }
             }
         }
@@ -481,7 +484,7 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
                 }
         __syncthreads();
         const int first = share_of(total, n_cta, seg0), last = share_of(total, n_cta, seg1 - 1);
-        const int rec = group * (2 + D);   // floats of a partial result
+        const int rec = 2 * PAGED_MAX_GROUP + group * D;   // floats of a partial result: m, l, o
         float* part = a.part + (2 * static_cast<size_t>(blockIdx.x) + (static_cast<int>(blockIdx.x) == first)) * rec;
         float* out = a.out + (static_cast<size_t>(seq) * g.n_head + kv * group) * D;
         float2* stats = a.stats + static_cast<size_t>(seq) * g.n_head + kv * group;
@@ -502,7 +505,7 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
                 out[i] = x * (1.0f / P_SCALE) * inv;
                 if (MASS && d == 0) stats[h] = make_float2(top, inv);
             } else {
-                part[2 * group + i] = x;
+                part[2 * PAGED_MAX_GROUP + i] = x;
                 if (d == 0) part[h] = top, part[group + h] = sum;
             }
         }
@@ -517,22 +520,39 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
             __syncthreads();
             if (s_last) {
                 __threadfence();
+                // Records in order of position.  Their maxima and sums are read first, the factors 2^(m_k - m)
+                // laid out in shared memory, and then every thread runs down the records with several loads in
+                // flight.
                 const int np = last - first + 1;
                 auto record = [&](int k) { return a.part + (2 * static_cast<size_t>(first + k) + (k == 0)) * rec; };
-                for (int i = tid; i < group * D; i += THREADS) {
-                    const int h = i / D, d = i % D;
-                    float top = -INFINITY, sum = 0.0f, x = 0.0f;
-                    for (int k = 0; k < np; ++k) top = fmaxf(top, __ldcg(record(k) + h));
-                    for (int k = 0; k < np; ++k) {
-                        const float* r = record(k);
-                        const float mk = __ldcg(r + h);
-                        const float e = mk == -INFINITY ? 0.0f : exp2f(mk - top);
-                        sum = fmaf(__ldcg(r + group + h), e, sum);
-                        x = fmaf(__ldcg(r + 2 * group + i), e, x);
+                float* ef = comb;   // [np][group] factors; np <= PAGED_MAX_CTAS
+                for (int h = warp; h < group; h += WARPS) {
+                    float top = -INFINITY, sum = 0.0f;
+                    for (int k = lane; k < np; k += 32) top = fmaxf(top, ef[k * group + h] = __ldcg(record(k) + h));
+                    for (int o2 = 16; o2 >= 1; o2 >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o2));
+                    for (int k = lane; k < np; k += 32) {
+                        const float mk = ef[k * group + h], e = mk == -INFINITY ? 0.0f : exp2f(mk - top);
+                        ef[k * group + h] = e;
+                        sum = fmaf(__ldcg(record(k) + group + h), e, sum);
                     }
-                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                    out[i] = x * (1.0f / P_SCALE) * inv;
-                    if (MASS && d == 0) stats[h] = make_float2(top, inv);
+                    for (int o2 = 16; o2 >= 1; o2 >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o2);
+                    if (lane == 0) {
+                        s_m[0][h] = sum == 0.0f ? 0.0f : 1.0f / sum;
+                        if (MASS) stats[h] = make_float2(top, s_m[0][h]);
+                    }
+                }
+                __syncthreads();
+                for (int i = tid; i < group * D / 4; i += THREADS) {
+                    const int h = 4 * i / D;
+                    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+                    for (int k = 0; k < np; ++k) {
+                        const float4 r = __ldcg(reinterpret_cast<const float4*>(record(k) + 2 * PAGED_MAX_GROUP) + i);
+                        const float e = ef[k * group + h];
+                        x = make_float4(fmaf(r.x, e, x.x), fmaf(r.y, e, x.y), fmaf(r.z, e, x.z), fmaf(r.w, e, x.w));
+                    }
+                    const float f = s_m[0][h] * (1.0f / P_SCALE);
+                    reinterpret_cast<float4*>(out)[i] = make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
                 }
             }
         }
@@ -563,15 +583,20 @@ __global__ void k_paged_mass(const PagedGeom g, const AttArgs a, float* __restri
 
 constexpr size_t up(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 size_t part_floats(const PagedGeom& g) {
-    return 2ull * PAGED_MAX_CTAS * (g.n_head / g.n_head_kv) * (2 + g.head_dim);
+    return 2ull * PAGED_MAX_CTAS * (2 * PAGED_MAX_GROUP + g.n_head / g.n_head_kv * g.head_dim);
 }
 
 template <typename T, int D, int NT, bool MASS>
-cudaError_t run(const PagedGeom& g, const AttArgs& a, float* mass, int n_sm, cudaStream_t s) {
+cudaError_t run(const PagedGeom& g, const AttArgs& a, float* mass, int dev, int n_sm, cudaStream_t s) {
     using L = Tile<T, D, NT>;
     auto* kernel = k_paged_attention<T, D, NT, MASS>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
-    if (e != cudaSuccess) return e;
+    static bool prepared[64] = {};   // per device: a repeated call sets the same value again
+    cudaError_t e;
+    if (!prepared[dev]) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM);
+        if (e != cudaSuccess) return e;
+        prepared[dev] = true;
+    }
     const int grid = std::min(n_sm * L::CTAS, PAGED_MAX_CTAS);
     kernel<<<grid, THREADS, L::SMEM, s>>>(g, a);
     e = cudaGetLastError();
@@ -585,13 +610,13 @@ cudaError_t run(const PagedGeom& g, const AttArgs& a, float* mass, int n_sm, cud
 }
 
 template <typename T>
-cudaError_t pick(const PagedGeom& g, const AttArgs& a, float* mass, int n_sm, cudaStream_t s) {
+cudaError_t pick(const PagedGeom& g, const AttArgs& a, float* mass, int dev, int n_sm, cudaStream_t s) {
     const bool two = a.group > 8;   // heads beside the 8 of one instruction
     if (g.head_dim == 64)
-        return mass ? (two ? run<T, 64, 2, true>(g, a, mass, n_sm, s) : run<T, 64, 1, true>(g, a, mass, n_sm, s))
-                    : (two ? run<T, 64, 2, false>(g, a, mass, n_sm, s) : run<T, 64, 1, false>(g, a, mass, n_sm, s));
-    return mass ? (two ? run<T, 128, 2, true>(g, a, mass, n_sm, s) : run<T, 128, 1, true>(g, a, mass, n_sm, s))
-                : (two ? run<T, 128, 2, false>(g, a, mass, n_sm, s) : run<T, 128, 1, false>(g, a, mass, n_sm, s));
+        return mass ? (two ? run<T, 64, 2, true>(g, a, mass, dev, n_sm, s) : run<T, 64, 1, true>(g, a, mass, dev, n_sm, s))
+                    : (two ? run<T, 64, 2, false>(g, a, mass, dev, n_sm, s) : run<T, 64, 1, false>(g, a, mass, dev, n_sm, s));
+    return mass ? (two ? run<T, 128, 2, true>(g, a, mass, dev, n_sm, s) : run<T, 128, 1, true>(g, a, mass, dev, n_sm, s))
+                : (two ? run<T, 128, 2, false>(g, a, mass, dev, n_sm, s) : run<T, 128, 1, false>(g, a, mass, dev, n_sm, s));
 }
 
 }  // namespace
@@ -624,9 +649,9 @@ cudaError_t launch_paged_attention(const PagedGeom& g, int kv_type, int max_seqs
     a.part = reinterpret_cast<float*>(w);
     w += up(sizeof(float) * part_floats(g));
     a.scores = reinterpret_cast<float*>(w);
-    if (kv_type == MCPM_KV_F32) return pick<float>(g, a, mass, n_sms[dev], s);
-    if (kv_type == MCPM_KV_F16) return pick<__half>(g, a, mass, n_sms[dev], s);
-    return pick<__nv_bfloat16>(g, a, mass, n_sms[dev], s);
+    if (kv_type == MCPM_KV_F32) return pick<float>(g, a, mass, dev, n_sms[dev], s);
+    if (kv_type == MCPM_KV_F16) return pick<__half>(g, a, mass, dev, n_sms[dev], s);
+    return pick<__nv_bfloat16>(g, a, mass, dev, n_sms[dev], s);
 }
 
 }  // namespace mcpm
