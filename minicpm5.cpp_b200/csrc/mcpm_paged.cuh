@@ -49,7 +49,7 @@ struct PagedGeom {
 };
 
 // Attention (mcpm_paged_attention.cu).
-constexpr int PAGED_MAX_CTAS = 320;   // most CTAs of a launch: sizes the workspace's partial results
+constexpr int PAGED_MAX_CTAS = 480;   // most CTAs of a launch: sizes the workspace's partial results
 size_t paged_attention_workspace(const PagedGeom& g, int max_seqs);
 cudaError_t launch_paged_attention(const PagedGeom& g, int kv_type, int max_seqs, const void* kc, const void* vc, float* mass,
                                    const int* table, const int* len, int n_seq, const float* q, long long q_stride, float* out,

@@ -29,7 +29,7 @@ namespace {
 constexpr int WARPS = 4, THREADS = 32 * WARPS;
 constexpr int ROWS = 16;            // positions of a warp's tile
 constexpr int UNIT = ROWS * WARPS;  // positions of a unit of work
-constexpr int MIN_UNITS = 2;        // units that a CTA takes before the next CTA is used
+constexpr int MIN_UNITS = 1;        // units that a CTA takes before the next CTA is used
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float P_SCALE = 1024.0f;  // weights are multiplied by this before they are split: fp16 parts of small
                                     // weights stay normal; undone in the output
@@ -55,7 +55,8 @@ struct Tile {
     static constexpr int CTAS = stages(112 * 1024) >= 3 ? 2 : 1;
     static constexpr int STAGES = stages((CTAS == 2 ? 112 : 224) * 1024);
     static constexpr int SMEM = WARPS * STAGES * STAGE + Q_BYTES;
-    static_assert(STAGES >= 2 && WARPS * 8 * NT * (D + 4) * 4 <= WARPS * STAGES * STAGE, "the rings hold the warps' outputs");
+    static_assert(STAGES >= 2 && 8 * NT * D * 4 <= STAGE - HEAD, "a slot holds a warp's output");
+    static_assert(PAGED_MAX_CTAS * PAGED_MAX_GROUP * 4 <= WARPS * STAGES * STAGE, "the rings hold the join's factors");
 };
 
 struct AttArgs {
@@ -96,13 +97,13 @@ __device__ __forceinline__ float4 lds_f4(uint32_t addr) {
 template <typename T>
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     if constexpr (sizeof(T) == 4)
-        asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     else if constexpr (__is_same(T, __half))
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     else
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
@@ -146,11 +147,10 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
     __shared__ long long s_sum[WARPS], s_base;
     __shared__ int s_seq, s_last;
     __shared__ float s_qf[8 * NT];              // scale of a head's scores in units of log2
-    __shared__ float s_m[WARPS][8 * NT], s_l[WARPS][8 * NT];
+    __shared__ float s_m[WARPS][8 * NT], s_l[WARPS][8 * NT], s_inv[8 * NT];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, t4 = lane & 3;
     uint32_t* qs = reinterpret_cast<uint32_t*>(smem + WARPS * L::STAGES * L::STAGE);
     uint8_t* ring = smem + warp * L::STAGES * L::STAGE;
-    float* comb = reinterpret_cast<float*>(smem);   // [warp][head][D + 4] once the rings are drained
     const T *kc = static_cast<const T*>(a.kc), *vc = static_cast<const T*>(a.vc);
     const int group = a.group, hkv = g.n_head_kv;
 
@@ -180,9 +180,10 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
         if (a.len[seq] <= 0)
             for (int i = tid; i < g.n_head * D; i += THREADS) a.out[static_cast<size_t>(seq) * g.n_head * D + i] = 0.0f;
     if (static_cast<int>(blockIdx.x) >= n_cta) return;
-    long long f = share_start(total, n_cta, blockIdx.x);
-    const long long f_end = share_start(total, n_cta, blockIdx.x + 1);
+    const long long f0 = share_start(total, n_cta, blockIdx.x);
+    const int n = static_cast<int>(share_start(total, n_cta, blockIdx.x + 1) - f0);   // units of this CTA
     {
+        const long long f = f0;
         long long base = before;
         if (f >= base && f < base + mine * hkv)
             for (int i = tid * per;; ++i) {
@@ -196,65 +197,138 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
             }
     }
     __syncthreads();
-    int seq = s_seq;
-    long long seq_base = s_base;   // first unit of the sequence
+    int seq = s_seq, units = units_of(seq);
+    int kv = static_cast<int>((f0 - s_base) / units), u = static_cast<int>((f0 - s_base) % units);
 
-    while (f < f_end) {
-        const int units = units_of(seq);
-        if (f >= seq_base + static_cast<long long>(units) * hkv) {
-            seq_base += static_cast<long long>(units) * hkv;
-            ++seq;
-            continue;
-        }
-        const int kv = static_cast<int>((f - seq_base) / units);
-        const long long seg0 = seq_base + static_cast<long long>(kv) * units, seg1 = seg0 + units;
-        const int u0 = static_cast<int>(f - seg0), u1 = static_cast<int>(min(seg1, f_end) - seg0);
-        f = min(seg1, f_end);
-        const int len = g.clamp_len(a.len[seq]);
-        const int* row = a.table + static_cast<size_t>(seq) * g.max_pages;
-
-        // ---- copies of K and V rows: lane & 15 looks a row of the tile up, all lanes copy
-        auto lookup = [&](int tile, int& page) {   // tile: this warp's tiles u0 .. u1 - 1
-            const int j = tile * UNIT + warp * ROWS + (lane & 15);
-            page = -1;
-            if (tile < u1 && j < len) page = __ldg(row + g.by_page.div(static_cast<uint32_t>(j)));
-        };
-        auto issue = [&](int tile, int page) {
-            if (tile < u1) {
-                uint8_t* st = ring + (tile - u0) % L::STAGES * L::STAGE;
-                const int j = tile * UNIT + warp * ROWS + (lane & 15);
-                const int slot = j - static_cast<int>(g.by_page.div(static_cast<uint32_t>(j))) * g.page_size;
-                const bool ok = static_cast<unsigned>(page) < static_cast<unsigned>(g.n_pages);
-                const long long off = ok ? g.row(page, slot, kv) : -1;
-                if (lane < 16) reinterpret_cast<int*>(st)[lane] = ok ? page * g.page_size + slot : -1;
-                const uint32_t kd = smem_u32(st + L::HEAD), vd = kd + ROWS * L::KP;
-#pragma unroll
-                for (int i = 0; i < ROWS * L::CHUNKS / 32; ++i) {
-                    const int r = i * (32 / L::CHUNKS) + lane / L::CHUNKS, c = lane % L::CHUNKS;
-                    const long long o = __shfl_sync(0xffffffffu, off, r);
-                    const size_t at = (o < 0 ? 0 : o) + c * (16 / sizeof(T));
-                    cp_async16_zfill(kd + r * L::KP + c * 16, kc + at, o < 0);
-                    cp_async16_zfill(vd + r * L::VP + c * 16, vc + at, o < 0);
-                }
+    // ---- copies of K and V rows, STAGES - 1 units ahead of the products whatever pair they belong to, so the
+    // memory does not idle where one pair ends and the next begins.  Lane & 15 looks one row of the warp's tile
+    // up a unit before its copy, all lanes copy.
+    struct Ahead {
+        int page, slot, kv;
+    };
+    int p_k = 0, p_seq = seq, p_kv = kv, p_u = u, p_units = units, p_len = g.clamp_len(a.len[seq]);
+    auto look = [&](Ahead& x) {
+        x = Ahead{-1, 0, p_kv};
+        if (p_k >= n) return;
+        const int j = p_u * UNIT + warp * ROWS + (lane & 15), c = static_cast<int>(g.by_page.div(static_cast<uint32_t>(j)));
+        x.slot = j - c * g.page_size;
+        if (j < p_len) x.page = __ldg(a.table + static_cast<size_t>(p_seq) * g.max_pages + c);
+        if (++p_k < n && ++p_u == p_units) {
+            p_u = 0;
+            if (++p_kv == hkv) {
+                p_kv = 0;
+                do p_len = g.clamp_len(a.len[++p_seq]);
+                while (p_len == 0);   // ends: p_k < n units are left
+                p_units = (p_len + UNIT - 1) / UNIT;
             }
-            cp_async_commit();
-        };
-        int next_page;
-#pragma unroll 1
-        for (int i = 0; i < L::STAGES - 1; ++i) {
-            int page;
-            lookup(u0 + i, page);
-            issue(u0 + i, page);
         }
-        lookup(u0 + L::STAGES - 1, next_page);
+    };
+    auto issue = [&](int k, const Ahead& x) {
+        if (k < n) {
+            uint8_t* st = ring + k % L::STAGES * L::STAGE;
+            const bool ok = static_cast<unsigned>(x.page) < static_cast<unsigned>(g.n_pages);
+            const long long off = ok ? g.row(x.page, x.slot, x.kv) : -1;
+            if (lane < 16) reinterpret_cast<int*>(st)[lane] = ok ? x.page * g.page_size + x.slot : -1;
+            const uint32_t kd = smem_u32(st + L::HEAD), vd = kd + ROWS * L::KP;
+#pragma unroll
+            for (int i = 0; i < ROWS * L::CHUNKS / 32; ++i) {
+                const int r = i * (32 / L::CHUNKS) + lane / L::CHUNKS, c = lane % L::CHUNKS;
+                const long long o = __shfl_sync(0xffffffffu, off, r);
+                const size_t at = (o < 0 ? 0 : o) + c * (16 / sizeof(T));
+                cp_async16_zfill(kd + r * L::KP + c * 16, kc + at, o < 0);
+                cp_async16_zfill(vd + r * L::VP + c * 16, vc + at, o < 0);
+            }
+        }
+        cp_async_commit();
+    };
+    // q of a pair: heads warp, warp + WARPS, ... of its group
+    float qx[2 * NT][D / 32];
+    auto load_q = [&](int q_seq, int q_kv) {
+#pragma unroll
+        for (int i = 0; i < 2 * NT; ++i) {
+            const int h = warp + WARPS * i;
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d)
+                qx[i][d] = h < group ? a.q[q_seq * a.q_stride + static_cast<size_t>(q_kv * group + h) * D + lane + 32 * d] : 0.0f;
+        }
+    };
+    Ahead next;
+    {
+        Ahead first[L::STAGES - 1];
+#pragma unroll
+        for (int i = 0; i < L::STAGES - 1; ++i) look(first[i]);
+        load_q(seq, kv);
+#pragma unroll
+        for (int i = 0; i < L::STAGES - 1; ++i) issue(i, first[i]);
+        look(next);
+    }
 
+    // ---- joins the records of a pair in order of position: their maxima and sums are read first, the factors
+    // 2^(m_k - m) laid out in shared memory, and then every thread runs down the records, several loads in flight
+    const int rec = 2 * PAGED_MAX_GROUP + group * D;   // floats of a record: m, l, o
+    auto finish = [&](int j_seq, int j_kv, int first, int last) {
+        const int np = last - first + 1;
+        auto record = [&](int k) { return a.part + (2 * static_cast<size_t>(first + k) + (k == 0)) * rec; };
+        float* ef = reinterpret_cast<float*>(smem);   // [np][group], np <= PAGED_MAX_CTAS; the rings are drained
+        float* out = a.out + (static_cast<size_t>(j_seq) * g.n_head + j_kv * group) * D;
+        for (int h = warp; h < group; h += WARPS) {
+            float top = -INFINITY, sum = 0.0f;
+            for (int k = lane; k < np; k += 32) {
+                const float mk = __ldcg(record(k) + h), lk = __ldcg(record(k) + PAGED_MAX_GROUP + h);
+                const float to = fmaxf(top, mk);
+                sum = fmaf(sum, top == -INFINITY ? 0.0f : exp2f(top - to), mk == -INFINITY ? 0.0f : lk * exp2f(mk - to));
+                top = to;
+                ef[k * group + h] = mk;
+            }
+            float all = top;
+            for (int o = 16; o >= 1; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
+            sum = top == -INFINITY ? 0.0f : sum * exp2f(top - all);
+            for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            for (int k = lane; k < np; k += 32) {
+                const float mk = ef[k * group + h];
+                ef[k * group + h] = mk == -INFINITY ? 0.0f : exp2f(mk - all);
+            }
+            if (lane == 0) {
+                s_inv[h] = sum == 0.0f ? 0.0f : 1.0f / sum;
+                if (MASS) a.stats[static_cast<size_t>(j_seq) * g.n_head + j_kv * group + h] = make_float2(all, s_inv[h]);
+            }
+        }
+        __syncthreads();
+        for (int i = tid; i < group * D / 4; i += THREADS) {
+            const int h = 4 * i / D;
+            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+            for (int k = 0; k < np; ++k) {
+                const float4 r = __ldcg(reinterpret_cast<const float4*>(record(k) + 2 * PAGED_MAX_GROUP) + i);
+                const float e = ef[k * group + h];
+                x = make_float4(fmaf(r.x, e, x.x), fmaf(r.y, e, x.y), fmaf(r.z, e, x.z), fmaf(r.w, e, x.w));
+            }
+            const float f = s_inv[h] * (1.0f / P_SCALE);
+            reinterpret_cast<float4*>(out)[i] = make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
+        }
+        __syncthreads();
+    };
+    // arrival at a pair that other CTAs share; only thread 0 has the answer
+    auto arrive = [&](int j_seq, int j_kv, int first, int last) {
+        unsigned* c = a.cnt + static_cast<size_t>(j_seq) * hkv + j_kv;
+        __threadfence();
+        const bool is_last = atomicAdd(c, 1u) == static_cast<unsigned>(last - first);
+        if (is_last) {
+            *c = 0u;
+            __threadfence();
+        }
+        return is_last;
+    };
+    int open_seq = -1, open_kv = 0, open_first = 0, open_last = 0;   // this CTA's first pair, if it began elsewhere
+    bool open_mine = false;
+
+    for (int k = 0; k < n;) {
         // ---- q in fragment order, normalised per head to [2^7, 2^8) so that 16-bit parts neither overflow
         // nor vanish
-        for (int h = warp; h < 8 * NT; h += WARPS) {
-            float x[D / 32];
 #pragma unroll
-            for (int i = 0; i < D / 32; ++i)
-                x[i] = h < group ? a.q[seq * a.q_stride + static_cast<size_t>(kv * group + h) * D + lane + 32 * i] : 0.0f;
+        for (int qi = 0; qi < 2 * NT; ++qi) {
+            const int h = warp + WARPS * qi;
+            const float(&x)[D / 32] = qx[qi];
             float top = 0.0f;
             for (int i = 0; i < D / 32; ++i) top = fmaxf(top, fabsf(x[i]));
             for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -295,12 +369,13 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
             for (int i = 0; i < D / 16; ++i) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.0f;
         }
 
-        for (int tile = u0; tile < u1; ++tile) {
+        const long long seg0 = f0 + k - u;   // the pair's first unit
+        for (const int k1 = min(n, k + units - u); k < k1; ++k) {
             cp_async_wait_group<L::STAGES - 2>();
-            __syncwarp();   // the tile is in shared memory for all lanes, and all are done with the slot that follows
-            issue(tile + L::STAGES - 1, next_page);
-            lookup(tile + L::STAGES, next_page);
-            const uint8_t* st = ring + (tile - u0) % L::STAGES * L::STAGE;
+            __syncwarp();   // the tile is in shared memory for all lanes, and all are done with the slot before it
+            issue(k + L::STAGES - 1, next);
+            look(next);
+            const uint8_t* st = ring + k % L::STAGES * L::STAGE;
             const int where0 = reinterpret_cast<const int*>(st)[gq], where1 = reinterpret_cast<const int*>(st)[gq + 8];
             const uint32_t ks = smem_u32(st + L::HEAD), vs = ks + ROWS * L::KP;
 
@@ -459,9 +534,26 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
                 }
             }
         }
-        cp_async_wait_all();
 
-        // ---- the CTA's result for this (sequence, KV head)
+        // ---- the next pair's q is on its way while this pair's result is put together
+        const int at_seq = seq, at_kv = kv;
+        const long long seg1 = seg0 + units;
+        if (k < n) {
+            u = 0;
+            if (++kv == hkv) {
+                kv = 0;
+                do units = units_of(++seq);
+                while (units == 0);
+            }
+            load_q(seq, kv);
+        }
+
+        // ---- the CTA's result for this (sequence, KV head): the slot that was read last holds the warp's output
+        auto comb = [&](int w) { return reinterpret_cast<float*>(smem + (w * L::STAGES + (k - 1) % L::STAGES) * L::STAGE + L::HEAD); };
+        auto swizzled = [&](int h, int d) {   // conflict-free stores of the accumulators' layout
+            return h * D + (d ^ ((h >> 1 & 3) * (sizeof(T) == 4 ? 1 : 8)));
+        };
+        __syncwarp();
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -472,7 +564,6 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
                 x += __shfl_xor_sync(0xffffffffu, x, 16);
                 if (gq == 0) s_m[warp][8 * nt + 2 * t4 + i] = m[nt][i], s_l[warp][8 * nt + 2 * t4 + i] = x;
             }
-        __syncthreads();   // rings are drained: their memory holds the warps' outputs now
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -480,83 +571,57 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int d = sizeof(T) == 4 ? 32 * (i / 2) + 4 * gq + 2 * (i & 1) + (e >> 1) : 16 * i + gq + 8 * (e >> 1);
-                    comb[((warp * NT + nt) * 8 + 2 * t4 + (e & 1)) * (D + 4) + d] = o[nt][i][e];
+                    comb(warp)[swizzled(8 * nt + 2 * t4 + (e & 1), d)] = o[nt][i][e];
                 }
         __syncthreads();
         const int first = share_of(total, n_cta, seg0), last = share_of(total, n_cta, seg1 - 1);
-        const int rec = 2 * PAGED_MAX_GROUP + group * D;   // floats of a partial result: m, l, o
         float* part = a.part + (2 * static_cast<size_t>(blockIdx.x) + (static_cast<int>(blockIdx.x) == first)) * rec;
-        float* out = a.out + (static_cast<size_t>(seq) * g.n_head + kv * group) * D;
-        float2* stats = a.stats + static_cast<size_t>(seq) * g.n_head + kv * group;
-        for (int i = tid; i < group * D; i += THREADS) {
-            const int h = i / D, d = i % D;
-            float top = s_m[0][h];
+        if (tid < group) {   // factors of the warps' outputs
+            float top = s_m[0][tid], sum = 0.0f;
 #pragma unroll
-            for (int w = 1; w < WARPS; ++w) top = fmaxf(top, s_m[w][h]);
-            float sum = 0.0f, x = 0.0f;
+            for (int w = 1; w < WARPS; ++w) top = fmaxf(top, s_m[w][tid]);
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) {
-                const float e = s_m[w][h] == -INFINITY ? 0.0f : exp2f(s_m[w][h] - top);
-                sum = fmaf(s_l[w][h], e, sum);
-                x = fmaf(comb[((w * NT + (h >> 3)) * 8 + (h & 7)) * (D + 4) + d], e, x);
+                const float e = s_m[w][tid] == -INFINITY ? 0.0f : exp2f(s_m[w][tid] - top);
+                sum = fmaf(s_l[w][tid], e, sum);
+                s_m[w][tid] = e;
             }
             if (first == last) {
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                out[i] = x * (1.0f / P_SCALE) * inv;
-                if (MASS && d == 0) stats[h] = make_float2(top, inv);
+                s_inv[tid] = inv * (1.0f / P_SCALE);
+                if (MASS) a.stats[static_cast<size_t>(at_seq) * g.n_head + at_kv * group + tid] = make_float2(top, inv);
             } else {
-                part[2 * PAGED_MAX_GROUP + i] = x;
-                if (d == 0) part[h] = top, part[group + h] = sum;
+                s_inv[tid] = 1.0f;
+                part[tid] = top;
+                part[PAGED_MAX_GROUP + tid] = sum;
             }
+        }
+        __syncthreads();
+        float* to = first == last ? a.out + (static_cast<size_t>(at_seq) * g.n_head + at_kv * group) * D : part + 2 * PAGED_MAX_GROUP;
+        for (int i = tid; i < group * D; i += THREADS) {
+            const int h = i / D, d = i % D;
+            float x = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) x = fmaf(comb(w)[swizzled(h, d)], s_m[w][h], x);
+            to[i] = x * s_inv[h];
         }
         if (first != last) {
-            __threadfence();
             __syncthreads();
-            if (tid == 0) {
-                unsigned* c = a.cnt + seq * hkv + kv;
-                s_last = atomicAdd(c, 1u) == static_cast<unsigned>(last - first);
-                if (s_last) *c = 0u;
-            }
-            __syncthreads();
-            if (s_last) {
-                __threadfence();
-                // Records in order of position.  Their maxima and sums are read first, the factors 2^(m_k - m)
-                // laid out in shared memory, and then every thread runs down the records with several loads in
-                // flight.
-                const int np = last - first + 1;
-                auto record = [&](int k) { return a.part + (2 * static_cast<size_t>(first + k) + (k == 0)) * rec; };
-                float* ef = comb;   // [np][group] factors; np <= PAGED_MAX_CTAS
-                for (int h = warp; h < group; h += WARPS) {
-                    float top = -INFINITY, sum = 0.0f;
-                    for (int k = lane; k < np; k += 32) top = fmaxf(top, ef[k * group + h] = __ldcg(record(k) + h));
-                    for (int o2 = 16; o2 >= 1; o2 >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o2));
-                    for (int k = lane; k < np; k += 32) {
-                        const float mk = ef[k * group + h], e = mk == -INFINITY ? 0.0f : exp2f(mk - top);
-                        ef[k * group + h] = e;
-                        sum = fmaf(__ldcg(record(k) + group + h), e, sum);
-                    }
-                    for (int o2 = 16; o2 >= 1; o2 >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o2);
-                    if (lane == 0) {
-                        s_m[0][h] = sum == 0.0f ? 0.0f : 1.0f / sum;
-                        if (MASS) stats[h] = make_float2(top, s_m[0][h]);
-                    }
-                }
+            if (k < n) {   // joined after this CTA's other pairs, so the arrival's round trip is not waited for
+                open_seq = at_seq, open_kv = at_kv, open_first = first, open_last = last;
+                if (tid == 0) open_mine = arrive(at_seq, at_kv, first, last);
+            } else {
+                if (tid == 0) s_last = arrive(at_seq, at_kv, first, last);
                 __syncthreads();
-                for (int i = tid; i < group * D / 4; i += THREADS) {
-                    const int h = 4 * i / D;
-                    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-                    for (int k = 0; k < np; ++k) {
-                        const float4 r = __ldcg(reinterpret_cast<const float4*>(record(k) + 2 * PAGED_MAX_GROUP) + i);
-                        const float e = ef[k * group + h];
-                        x = make_float4(fmaf(r.x, e, x.x), fmaf(r.y, e, x.y), fmaf(r.z, e, x.z), fmaf(r.w, e, x.w));
-                    }
-                    const float f = s_m[0][h] * (1.0f / P_SCALE);
-                    reinterpret_cast<float4*>(out)[i] = make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
-                }
+                if (s_last) finish(at_seq, at_kv, first, last);
             }
         }
-        __syncthreads();   // comb and s_m are free for the next pair
+    }
+    if (open_seq >= 0) {
+        __syncthreads();
+        if (tid == 0) s_last = open_mine;
+        __syncthreads();
+        if (s_last) finish(open_seq, open_kv, open_first, open_last);
     }
 }
 
