@@ -29,7 +29,12 @@ namespace {
 constexpr int WARPS = 4, THREADS = 32 * WARPS;
 constexpr int ROWS = 16;            // positions of a warp's tile
 constexpr int UNIT = ROWS * WARPS;  // positions of a unit of work
-constexpr int MIN_UNITS = 1;        // units that a CTA takes before the next CTA is used
+constexpr int FAN = 8, FAN_BITS = 3, LEVELS = 3;   // records joined at a time, FAN^LEVELS >= PAGED_MAX_CTAS
+// Ends of shares move to a pair's end where the rest would cost more as a record, with its arrival and join,
+// than as work: inside pairs of at most WHOLE units always, else within `slack` units of an end (a quarter of a
+// share, at most 2).
+constexpr int WHOLE = 4;
+__device__ __forceinline__ int slack_of(long long total, int n) { return static_cast<int>(min(2LL, total / n / 4)); }
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float P_SCALE = 1024.0f;  // weights are multiplied by this before they are split: fp16 parts of small
                                     // weights stay normal; undone in the output
@@ -56,7 +61,6 @@ struct Tile {
     static constexpr int STAGES = stages((CTAS == 2 ? 112 : 224) * 1024);
     static constexpr int SMEM = WARPS * STAGES * STAGE + Q_BYTES;
     static_assert(STAGES >= 2 && 8 * NT * D * 4 <= STAGE - HEAD, "a slot holds a warp's output");
-    static_assert(PAGED_MAX_CTAS * PAGED_MAX_GROUP * 4 <= WARPS * STAGES * STAGE, "the rings hold the join's factors");
 };
 
 struct AttArgs {
@@ -67,7 +71,7 @@ struct AttArgs {
     float* out;
     float scale;
     int n_seq, group;
-    unsigned* cnt;     // [seq][kv head] arrivals, zero between calls
+    unsigned* cnt;     // [LEVELS][slot of the first record] arrivals, zero between calls
     float2* stats;     // [seq][head] (max in units of log2, 1 / sum); mass only
     float* part;       // [2 CTA + which][m[group], l[group], pad to 32, o[group][D]]
     float* scores;     // [page * page_size + slot][n_head] scores in units of log2; mass only
@@ -144,8 +148,8 @@ template <typename T, int D, int NT, bool MASS>
 __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attention(const PagedGeom g, const AttArgs a) {
     using L = Tile<T, D, NT>;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ long long s_sum[WARPS], s_base;
-    __shared__ int s_seq, s_last;
+    __shared__ long long s_sum[WARPS], s_at[2];
+    __shared__ int s_seq, s_kv, s_u, s_last;
     __shared__ float s_qf[8 * NT];              // scale of a head's scores in units of log2
     __shared__ float s_m[WARPS][8 * NT], s_l[WARPS][8 * NT], s_inv[8 * NT];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gq = lane >> 2, t4 = lane & 3;
@@ -154,6 +158,8 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
     const T *kc = static_cast<const T*>(a.kc), *vc = static_cast<const T*>(a.vc);
     const int group = a.group, hkv = g.n_head_kv;
 
+    grid_dep_launch();
+    grid_dep_wait();
     // ---- this CTA's share of the units
     auto units_of = [&](int seq) { return (g.clamp_len(a.len[seq]) + UNIT - 1) / UNIT; };
     const int per = (a.n_seq + THREADS - 1) / THREADS;
@@ -174,31 +180,42 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
     }
     before = (before - mine) * hkv;
     total *= hkv;
-    const int n_cta = static_cast<int>(min(static_cast<long long>(gridDim.x), (total + MIN_UNITS - 1) / MIN_UNITS));
+    const int n_cta = static_cast<int>(min(static_cast<long long>(gridDim.x), total));
     // sequences without positions: zeros
     for (int seq = blockIdx.x; seq < a.n_seq; seq += gridDim.x)
         if (a.len[seq] <= 0)
             for (int i = tid; i < g.n_head * D; i += THREADS) a.out[static_cast<size_t>(seq) * g.n_head * D + i] = 0.0f;
     if (static_cast<int>(blockIdx.x) >= n_cta) return;
-    const long long f0 = share_start(total, n_cta, blockIdx.x);
-    const int n = static_cast<int>(share_start(total, n_cta, blockIdx.x + 1) - f0);   // units of this CTA
-    {
-        const long long f = f0;
+    // where this share begins and the next one does
+    const int slack = slack_of(total, n_cta);
+    for (int side = 0; side < 2; ++side) {
+        const long long f = share_start(total, n_cta, blockIdx.x + side);
         long long base = before;
+        if (f == total && tid == 0 && side) s_at[1] = total;
         if (f >= base && f < base + mine * hkv)
             for (int i = tid * per;; ++i) {
-                const long long n = static_cast<long long>(units_of(i)) * hkv;
-                if (f < base + n) {
-                    s_seq = i;
-                    s_base = base;
+                const int units = units_of(i);
+                if (f < base + static_cast<long long>(units) * hkv) {
+                    const int kv = static_cast<int>((f - base) / units), u = static_cast<int>((f - base) % units);
+                    const bool near = units <= WHOLE || min(u, units - u) <= slack, down = near && u <= units - u, up = near && !down;
+                    s_at[side] = down ? f - u : up ? f - u + units : f;
+                    if (side == 0) s_seq = i, s_kv = kv + up, s_u = down || up ? 0 : u;
                     break;
                 }
-                base += n;
+                base += static_cast<long long>(units) * hkv;
             }
     }
     __syncthreads();
-    int seq = s_seq, units = units_of(seq);
-    int kv = static_cast<int>((f0 - s_base) / units), u = static_cast<int>((f0 - s_base) % units);
+    const long long f0 = s_at[0];
+    const int n = static_cast<int>(s_at[1] - f0);   // units of this CTA
+    if (n <= 0) return;
+    int seq = s_seq, kv = s_kv, u = s_u;
+    if (kv == hkv) {
+        kv = 0;
+        do ++seq;
+        while (units_of(seq) == 0);   // ends: n > 0 units follow
+    }
+    int units = units_of(seq);
 
     // ---- copies of K and V rows, STAGES - 1 units ahead of the products whatever pair they belong to, so the
     // memory does not idle where one pair ends and the next begins.  Lane & 15 looks one row of the warp's tile
@@ -263,64 +280,77 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
         look(next);
     }
 
-    // ---- joins the records of a pair in order of position: their maxima and sums are read first, the factors
-    // 2^(m_k - m) laid out in shared memory, and then every thread runs down the records, several loads in flight
-    const int rec = 2 * PAGED_MAX_GROUP + group * D;   // floats of a record: m, l, o
-    auto finish = [&](int j_seq, int j_kv, int first, int last) {
-        const int np = last - first + 1;
-        auto record = [&](int k) { return a.part + (2 * static_cast<size_t>(first + k) + (k == 0)) * rec; };
-        float* ef = reinterpret_cast<float*>(smem);   // [np][group], np <= PAGED_MAX_CTAS; the rings are drained
-        float* out = a.out + (static_cast<size_t>(j_seq) * g.n_head + j_kv * group) * D;
-        for (int h = warp; h < group; h += WARPS) {
-            float top = -INFINITY, sum = 0.0f;
-            for (int k = lane; k < np; k += 32) {
-                const float mk = __ldcg(record(k) + h), lk = __ldcg(record(k) + PAGED_MAX_GROUP + h);
-                const float to = fmaxf(top, mk);
-                sum = fmaf(sum, top == -INFINITY ? 0.0f : exp2f(top - to), mk == -INFINITY ? 0.0f : lk * exp2f(mk - to));
-                top = to;
-                ef[k * group + h] = mk;
-            }
-            float all = top;
-            for (int o = 16; o >= 1; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
-            sum = top == -INFINITY ? 0.0f : sum * exp2f(top - all);
-            for (int o = 16; o >= 1; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            for (int k = lane; k < np; k += 32) {
-                const float mk = ef[k * group + h];
-                ef[k * group + h] = mk == -INFINITY ? 0.0f : exp2f(mk - all);
-            }
-            if (lane == 0) {
-                s_inv[h] = sum == 0.0f ? 0.0f : 1.0f / sum;
-                if (MASS) a.stats[static_cast<size_t>(j_seq) * g.n_head + j_kv * group + h] = make_float2(all, s_inv[h]);
-            }
-        }
-        __syncthreads();
-        for (int i = tid; i < group * D / 4; i += THREADS) {
-            const int h = 4 * i / D;
-            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-            for (int k = 0; k < np; ++k) {
-                const float4 r = __ldcg(reinterpret_cast<const float4*>(record(k) + 2 * PAGED_MAX_GROUP) + i);
-                const float e = ef[k * group + h];
-                x = make_float4(fmaf(r.x, e, x.x), fmaf(r.y, e, x.y), fmaf(r.z, e, x.z), fmaf(r.w, e, x.w));
-            }
-            const float f = s_inv[h] * (1.0f / P_SCALE);
-            reinterpret_cast<float4*>(out)[i] = make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
-        }
-        __syncthreads();
-    };
-    // arrival at a pair that other CTAs share; only thread 0 has the answer
-    auto arrive = [&](int j_seq, int j_kv, int first, int last) {
-        unsigned* c = a.cnt + static_cast<size_t>(j_seq) * hkv + j_kv;
+    // ---- A pair of several CTAs leaves a record (m, l, o) per CTA.  Records are joined eight at a time, in order
+    // of position, by the CTA that arrives last at the eight; its result is a record of the next level, and the
+    // last level's is the output.  One CTA reading all records of a long sequence took 7 us of a 20 us call.
+    const int rec = 2 * PAGED_MAX_GROUP + group * D;   // floats of a record
+    auto arrive = [&](int level, int slot, int members) {   // thread 0, after the CTA's stores and a barrier
+        unsigned* c = a.cnt + level * 2 * PAGED_MAX_CTAS + slot;
         __threadfence();
-        const bool is_last = atomicAdd(c, 1u) == static_cast<unsigned>(last - first);
-        if (is_last) {
-            *c = 0u;
-            __threadfence();
-        }
-        return is_last;
+        const bool last = atomicAdd(c, 1u) == static_cast<unsigned>(members - 1);
+        if (last) *c = 0u;
+        __threadfence();
+        return last;
     };
-    int open_seq = -1, open_kv = 0, open_first = 0, open_last = 0;   // this CTA's first pair, if it began elsewhere
-    bool open_mine = false;
+    struct Shared {   // a pair of CTAs first .. first + np - 1, this one's record being the k-th
+        int seq, kv, first, np, k;
+    };
+    auto slot_of = [](const Shared& s, int k) { return 2 * (s.first + k) + (k == 0); };   // a CTA begins one pair at most
+    auto members_of = [](const Shared& s, int level) {
+        const int step = 1 << FAN_BITS * level, at = s.k >> FAN_BITS * (level + 1) << FAN_BITS * (level + 1);
+        return min(FAN, (s.np - at + step - 1) >> FAN_BITS * level);
+    };
+    auto join = [&](Shared s) {   // s_last: whether this CTA arrived last at its first eight
+        for (int level = 0; s_last; ++level) {
+            const int at = s.k >> FAN_BITS * (level + 1) << FAN_BITS * (level + 1), members = members_of(s, level);
+            const bool done = s.np <= 1 << FAN_BITS * (level + 1);
+            float* to = a.part + static_cast<size_t>(slot_of(s, at)) * rec;
+            float* out = a.out + (static_cast<size_t>(s.seq) * g.n_head + s.kv * group) * D;
+            for (int i0 = 32 * warp; i0 < group * D / 4; i0 += THREADS) {   // whole warps: a head's items are one warp's
+                const int i = min(i0 + lane, group * D / 4 - 1), h = 4 * i / D;
+                const bool mine = i == i0 + lane;
+                float mr[FAN], lr[FAN];
+                float4 r[FAN];
+#pragma unroll
+                for (int j = 0; j < FAN; ++j)
+                    if (j < members) {
+                        const float* p = a.part + static_cast<size_t>(slot_of(s, at + (j << FAN_BITS * level))) * rec;
+                        mr[j] = __ldcg(p + h);
+                        lr[j] = __ldcg(p + PAGED_MAX_GROUP + h);
+                        r[j] = __ldcg(reinterpret_cast<const float4*>(p + 2 * PAGED_MAX_GROUP) + i);
+                    }
+                float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+                for (int j = 0; j < FAN; ++j)
+                    if (j < members) top = fmaxf(top, mr[j]);
+                float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int j = 0; j < FAN; ++j)
+                    if (j < members) {
+                        const float e = mr[j] == -INFINITY ? 0.0f : exp2f(mr[j] - top);
+                        sum = fmaf(lr[j], e, sum);
+                        x = make_float4(fmaf(r[j].x, e, x.x), fmaf(r[j].y, e, x.y), fmaf(r[j].z, e, x.z), fmaf(r[j].w, e, x.w));
+                    }
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum, f = done ? inv * (1.0f / P_SCALE) : 1.0f;
+                const float4 y = make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
+                if (done) {
+                    if (mine) reinterpret_cast<float4*>(out)[i] = y;
+                    if (MASS && mine && 4 * i % D == 0) a.stats[static_cast<size_t>(s.seq) * g.n_head + s.kv * group + h] = make_float2(top, inv);
+                } else {
+                    __syncwarp();   // the record is joined in place: all lanes have read it
+                    if (mine) reinterpret_cast<float4*>(to + 2 * PAGED_MAX_GROUP)[i] = y;
+                    if (mine && 4 * i % D == 0) to[h] = top, to[PAGED_MAX_GROUP + h] = sum;
+                }
+            }
+            __syncthreads();
+            if (done) break;
+            s.k = at;
+            if (tid == 0) s_last = arrive(level + 1, slot_of(s, s.k >> FAN_BITS * (level + 2) << FAN_BITS * (level + 2)), members_of(s, level + 1));
+            __syncthreads();
+        }
+    };
+    Shared open{-1, 0, 0, 0, 0};   // this CTA's first pair, if other CTAs share it
+    bool open_last = false;
 
     for (int k = 0; k < n;) {
         // ---- q in fragment order, normalised per head to [2^7, 2^8) so that 16-bit parts neither overflow
@@ -381,11 +411,14 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
 
             // ---- scores
             // Independent accumulators: the instruction truncates, so short chains lose less, and they overlap.
-            float s[NT][4], s_hi[NT][2][4], s_lo[NT][4];
+            float s[NT][4], s_hi[NT][2][4], s_lo[NT][4][4];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s_hi[nt][0][i] = s_hi[nt][1][i] = s_lo[nt][i] = 0.0f;
+                for (int i = 0; i < 4; ++i) {
+                    s_hi[nt][0][i] = s_hi[nt][1][i] = 0.0f;
+                    s_lo[nt][0][i] = s_lo[nt][1][i] = s_lo[nt][2][i] = s_lo[nt][3][i] = 0.0f;
+                }
             if constexpr (sizeof(T) == 4) {
 #pragma unroll
                 for (int c = 0; c < D / 16; ++c) {
@@ -406,8 +439,8 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
                         for (int nt = 0; nt < NT; ++nt) {
                             const uint4 b = *reinterpret_cast<const uint4*>(qs + (((2 * c + k) * NT + nt) * 32 + lane) * 4);
                             mma<T>(s_hi[nt][k], hi[k], b.x, b.y);
-                            mma<T>(s_lo[nt], hi[k], b.z, b.w);
-                            mma<T>(s_lo[nt], lo[k], b.x, b.y);
+                            mma<T>(s_lo[nt][k], hi[k], b.z, b.w);
+                            mma<T>(s_lo[nt][2 + k], lo[k], b.x, b.y);
                         }
                 }
             } else {
@@ -420,7 +453,7 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
                         const uint2* b = reinterpret_cast<const uint2*>(qs + ((c * NT + nt) * 32 + lane) * L::QWORDS);
                         mma<T>(s_hi[nt][c & 1], k, b[0].x, b[0].y);
 #pragma unroll
-                        for (int p = 1; p < parts<T>(); ++p) mma<T>(s_lo[nt], k, b[p].x, b[p].y);
+                        for (int p = 1; p < parts<T>(); ++p) mma<T>(s_lo[nt][2 * (p - 1) + (c & 1)], k, b[p].x, b[p].y);
                     }
                 }
             }
@@ -429,7 +462,8 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[nt][i] = s_hi[nt][0][i] + s_hi[nt][1][i] + s_lo[nt][i];
+                for (int i = 0; i < 4; ++i)
+                    s[nt][i] = s_hi[nt][0][i] + s_hi[nt][1][i] + ((s_lo[nt][0][i] + s_lo[nt][1][i]) + (s_lo[nt][2][i] + s_lo[nt][3][i]));
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const float x = where0 >= 0 ? s[nt][i] * qf[nt][i] : -INFINITY;
@@ -574,8 +608,8 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
                     comb(warp)[swizzled(8 * nt + 2 * t4 + (e & 1), d)] = o[nt][i][e];
                 }
         __syncthreads();
-        const int first = share_of(total, n_cta, seg0), last = share_of(total, n_cta, seg1 - 1);
-        float* part = a.part + (2 * static_cast<size_t>(blockIdx.x) + (static_cast<int>(blockIdx.x) == first)) * rec;
+        const bool whole = seg0 >= f0 && seg1 <= f0 + n;
+        float* part = a.part + (2 * static_cast<size_t>(blockIdx.x) + (seg0 >= f0)) * rec;
         if (tid < group) {   // factors of the warps' outputs
             float top = s_m[0][tid], sum = 0.0f;
 #pragma unroll
@@ -586,7 +620,7 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
                 sum = fmaf(s_l[w][tid], e, sum);
                 s_m[w][tid] = e;
             }
-            if (first == last) {
+            if (whole) {
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
                 s_inv[tid] = inv * (1.0f / P_SCALE);
                 if (MASS) a.stats[static_cast<size_t>(at_seq) * g.n_head + at_kv * group + tid] = make_float2(top, inv);
@@ -597,7 +631,7 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
             }
         }
         __syncthreads();
-        float* to = first == last ? a.out + (static_cast<size_t>(at_seq) * g.n_head + at_kv * group) * D : part + 2 * PAGED_MAX_GROUP;
+        float* to = whole ? a.out + (static_cast<size_t>(at_seq) * g.n_head + at_kv * group) * D : part + 2 * PAGED_MAX_GROUP;
         for (int i = tid; i < group * D; i += THREADS) {
             const int h = i / D, d = i % D;
             float x = 0.0f;
@@ -605,48 +639,54 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
             for (int w = 0; w < WARPS; ++w) x = fmaf(comb(w)[swizzled(h, d)], s_m[w][h], x);
             to[i] = x * s_inv[h];
         }
-        if (first != last) {
+        if (!whole) {
+            // shares whose (moved) ends lie in this pair
+            const int first = share_of(total, n_cta, seg0 + slack), last = share_of(total, n_cta, seg1 - 1 - slack);
+            const Shared s{at_seq, at_kv, first, last - first + 1, static_cast<int>(blockIdx.x) - first};
             __syncthreads();
             if (k < n) {   // joined after this CTA's other pairs, so the arrival's round trip is not waited for
-                open_seq = at_seq, open_kv = at_kv, open_first = first, open_last = last;
-                if (tid == 0) open_mine = arrive(at_seq, at_kv, first, last);
+                open = s;
+                if (tid == 0) open_last = arrive(0, slot_of(s, s.k & ~(FAN - 1)), members_of(s, 0));
             } else {
-                if (tid == 0) s_last = arrive(at_seq, at_kv, first, last);
+                if (tid == 0) s_last = arrive(0, slot_of(s, s.k & ~(FAN - 1)), members_of(s, 0));
                 __syncthreads();
-                if (s_last) finish(at_seq, at_kv, first, last);
+                join(s);
             }
         }
     }
-    if (open_seq >= 0) {
+    if (open.seq >= 0) {
         __syncthreads();
-        if (tid == 0) s_last = open_mine;
+        if (tid == 0) s_last = open_last;
         __syncthreads();
-        if (s_last) finish(open_seq, open_kv, open_first, open_last);
+        join(open);
     }
 }
 
-// mass[position] += sum over the KV head's query heads of exp(s - max) / sum.  A thread per (position,
-// KV head); grid.y sequences, grid.x equal shares of a sequence.
-__global__ void k_paged_mass(const PagedGeom g, const AttArgs a, float* __restrict__ mass) {
-    extern __shared__ float2 st[];
+// mass[position] += sum over the KV head's query heads of exp(s - max) / sum.  A warp per 32 positions of a KV
+// head; grid.y sequences.
+constexpr int MASS_WARPS = 8;
+__global__ void __launch_bounds__(32 * MASS_WARPS) k_paged_mass(const PagedGeom g, const AttArgs a, float* __restrict__ mass) {
+    grid_dep_launch();
     grid_dep_wait();
-    const int seq = blockIdx.y, n = g.clamp_len(a.len[seq]), hkv = g.n_head_kv;
-    for (int i = threadIdx.x; i < g.n_head; i += blockDim.x) st[i] = a.stats[static_cast<size_t>(seq) * g.n_head + i];
-    __syncthreads();
+    const int seq = blockIdx.y, n = g.clamp_len(a.len[seq]), hkv = g.n_head_kv, lane = threadIdx.x & 31;
     const int* row = a.table + static_cast<size_t>(seq) * g.max_pages;
-    const long long items = static_cast<long long>(n) * hkv;
-    for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < items; i += static_cast<long long>(gridDim.x) * blockDim.x) {
-        const int j = static_cast<int>(i / hkv), kv = static_cast<int>(i % hkv);
+    const int tiles = (n + 31) / 32;
+    for (int w = blockIdx.x * MASS_WARPS + (threadIdx.x >> 5); w < tiles; w += gridDim.x * MASS_WARPS) {
+        const int j = 32 * w + lane;
         int page, slot;
-        if (!g.locate(row, j, page, slot)) continue;
-        const float* s = a.scores + (static_cast<size_t>(page) * g.page_size + slot) * g.n_head + kv * a.group;
-        float w = 0.0f;
-        for (int h = 0; h < a.group; ++h) w = fmaf(exp2f(s[h] - st[kv * a.group + h].x), st[kv * a.group + h].y, w);
-        mass[g.mass_at(page, slot, kv)] += w;
+        if (j >= n || !g.locate(row, j, page, slot)) continue;
+        const float* s = a.scores + (static_cast<size_t>(page) * g.page_size + slot) * g.n_head;
+        const float2* st = a.stats + static_cast<size_t>(seq) * g.n_head;
+        for (int kv = 0; kv < hkv; ++kv) {
+            float x = 0.0f;
+            for (int h = kv * a.group; h < (kv + 1) * a.group; ++h) x = fmaf(exp2f(s[h] - st[h].x), st[h].y, x);
+            mass[g.mass_at(page, slot, kv)] += x;
+        }
     }
 }
 
 constexpr size_t up(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
+constexpr size_t COUNTERS = sizeof(unsigned) * LEVELS * 2 * PAGED_MAX_CTAS;
 size_t part_floats(const PagedGeom& g) {
     return 2ull * PAGED_MAX_CTAS * (2 * PAGED_MAX_GROUP + g.n_head / g.n_head_kv * g.head_dim);
 }
@@ -662,16 +702,11 @@ cudaError_t run(const PagedGeom& g, const AttArgs& a, float* mass, int dev, int 
         if (e != cudaSuccess) return e;
         prepared[dev] = true;
     }
-    const int grid = std::min(n_sm * L::CTAS, PAGED_MAX_CTAS);
-    kernel<<<grid, THREADS, L::SMEM, s>>>(g, a);
-    e = cudaGetLastError();
+    e = launch_dependent(kernel, dim3(std::min(n_sm * L::CTAS, PAGED_MAX_CTAS)), THREADS, L::SMEM, s, g, a);
     if (e != cudaSuccess || !MASS) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(std::max(1, (4 * n_sm + a.n_seq - 1) / a.n_seq), a.n_seq);
-    cfg.blockDim = dim3(256);
-    cfg.dynamicSmemBytes = g.n_head * sizeof(float2);
-    cfg.stream = s;
-    return cudaLaunchKernelEx(&cfg, k_paged_mass, g, a, mass);
+    const long long tiles = (static_cast<long long>(g.max_pages) * g.page_size + 31) / 32;
+    const long long blocks = std::min<long long>((tiles + MASS_WARPS - 1) / MASS_WARPS, std::max(1, 16 * n_sm / a.n_seq));
+    return launch_dependent(k_paged_mass, dim3(static_cast<unsigned>(blocks), a.n_seq), 32 * MASS_WARPS, 0, s, g, a, mass);
 }
 
 template <typename T>
@@ -687,8 +722,8 @@ cudaError_t pick(const PagedGeom& g, const AttArgs& a, float* mass, int dev, int
 }  // namespace
 
 size_t paged_attention_workspace(const PagedGeom& g, int max_seqs) {
-    return up(sizeof(unsigned) * max_seqs * g.n_head_kv) + up(sizeof(float2) * max_seqs * g.n_head) +
-           up(sizeof(float) * part_floats(g)) + sizeof(float) * static_cast<size_t>(g.n_pages) * g.page_size * g.n_head;
+    return up(COUNTERS) + up(sizeof(float2) * max_seqs * g.n_head) + up(sizeof(float) * part_floats(g)) +
+           sizeof(float) * static_cast<size_t>(g.n_pages) * g.page_size * g.n_head;
 }
 
 cudaError_t launch_paged_attention(const PagedGeom& g, int kv_type, int max_seqs, const void* kc, const void* vc, float* mass,
@@ -708,7 +743,7 @@ cudaError_t launch_paged_attention(const PagedGeom& g, int kv_type, int max_seqs
     uint8_t* w = static_cast<uint8_t*>(ws);
     AttArgs a{kc, vc, table, len, q, q_stride, out, scale, n_seq, g.n_head / g.n_head_kv};
     a.cnt = reinterpret_cast<unsigned*>(w);
-    w += up(sizeof(unsigned) * max_seqs * g.n_head_kv);
+    w += up(COUNTERS);
     a.stats = reinterpret_cast<float2*>(w);
     w += up(sizeof(float2) * max_seqs * g.n_head);
     a.part = reinterpret_cast<float*>(w);
