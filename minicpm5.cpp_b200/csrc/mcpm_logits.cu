@@ -13,7 +13,8 @@ namespace {
 
 constexpr int LG_CLUSTER = 8;        // CTAs that share a row
 constexpr int LG_THREADS = 512;
-constexpr int LG_SLICE = 16384;      // tokens whose counters a CTA holds at once (one word each)
+constexpr int LG_HELD = 32;          // logits a thread holds at once
+constexpr int LG_SLICE = LG_THREADS * LG_HELD;   // tokens whose counters a CTA holds at once (one word each)
 constexpr int LG_COUNT_BITS = 20;    // counter word: times in the history; above: last bias entry + 1
 constexpr int LG_MAX_HIST = (1 << LG_COUNT_BITS) - 1, LG_MAX_BIAS = (1 << (32 - LG_COUNT_BITS)) - 2;
 
@@ -26,15 +27,21 @@ __device__ __forceinline__ void take(Best& a, const Best& b) {
     if (b.v > a.v || (b.v == a.v && b.t < a.t)) a = b;
 }
 
-// A cluster of LG_CLUSTER CTAs per row, each with a contiguous share of the vocabulary.  The history
-// is counted into shared-memory words (integer atomics: the order does not matter), a bias entry
-// leaves its index there (the largest, hence the last entry, stays), and the logits stream past them.
-__global__ void __launch_bounds__(LG_THREADS) k_logits(const mcpm_logits_params p) {
-    extern __shared__ uint32_t words[];
+// A cluster of LG_CLUSTER CTAs per row, each with a contiguous share of the vocabulary, LG_SLICE tokens at a
+// time.  The slice's logits are on their way to registers while the history is counted into shared-memory
+// words (integer atomics: the order does not matter) and each bias entry leaves its index there (the largest,
+// hence the last entry, stays).  Tokens without a word go through at once, only masked.  The others are few:
+// the lists are walked again, and whoever takes a token's word first treats it, so no warp of the streaming
+// pass waits for one lane's division.  VEC = 4 where all rows are 16-byte aligned, else 1.
+template <int VEC>
+__global__ void __launch_bounds__(LG_THREADS, 2) k_logits(const mcpm_logits_params p) {
+    extern __shared__ __align__(16) uint32_t words[];
     __shared__ Best warp_best[LG_THREADS / 32], cta_best[LG_CLUSTER];
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     if (p.argmax) cluster.barrier_arrive();   // waited for before the first write to another CTA's memory
+    grid_dep_launch();
+    grid_dep_wait();
     const int tid = threadIdx.x, rank = cluster.block_rank(), row = blockIdx.x / LG_CLUSTER;
     const int share = ((p.n_vocab + LG_CLUSTER - 1) / LG_CLUSTER + 31) & ~31;   // whole mask words
     const int lo = min(p.n_vocab, rank * share), hi = min(p.n_vocab, lo + share);
@@ -45,55 +52,100 @@ __global__ void __launch_bounds__(LG_THREADS) k_logits(const mcpm_logits_params 
     const int* bias_token = p.bias_token ? p.bias_token + row * p.bias_stride : nullptr;
     const int n_bias = bias_token ? (p.bias_len ? min(max(p.bias_len[row], 0), p.bias_max) : p.bias_max) : 0;
     const uint32_t* allow = p.allow ? p.allow + row * p.allow_stride : nullptr;
+    const bool lists = n_hist || n_bias;
     float rep = 1.0f, freq = 0.0f, pres = 0.0f;
     if (n_hist) rep = p.penalties[3 * row], freq = p.penalties[3 * row + 1], pres = p.penalties[3 * row + 2];
     Best best{-INFINITY, 0x7fffffff};
+    auto consider = [&](float v, int t) {   // the lowest token of the largest value, whatever the order of calls
+        if (v > best.v || (v == best.v && t < best.t && v > -INFINITY)) best = Best{v, t};
+    };
+    auto allowed = [&](int t) { return !allow || (allow[t >> 5] >> (t & 31) & 1u); };
     for (int s0 = lo; s0 < hi; s0 += LG_SLICE) {
         const int n = min(LG_SLICE, hi - s0);
-        if (n_hist || n_bias) {
-            for (int i = tid; i < n; i += LG_THREADS) words[i] = 0u;
+        float v[LG_HELD];
+        if constexpr (VEC == 4) {
+#pragma unroll
+            for (int k = 0; k < LG_HELD / 4; ++k) {
+                const int i = 4 * (k * LG_THREADS + tid);
+                if (i + 3 < n)
+                    *reinterpret_cast<float4*>(v + 4 * k) = *reinterpret_cast<const float4*>(x + s0 + i);
+                else
+                    for (int e = 0; e < 4; ++e) v[4 * k + e] = i + e < n ? x[s0 + i + e] : 0.0f;
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < LG_HELD; ++k) v[k] = k * LG_THREADS + tid < n ? x[s0 + k * LG_THREADS + tid] : 0.0f;
+        }
+        if (lists) {
+            for (int i = tid; i < (n + 3) / 4; i += LG_THREADS) reinterpret_cast<uint4*>(words)[i] = make_uint4(0u, 0u, 0u, 0u);
             __syncthreads();
             for (int i = tid; i < n_bias; i += LG_THREADS) {
                 const unsigned t = static_cast<unsigned>(bias_token[i]) - static_cast<unsigned>(s0);
                 if (t < static_cast<unsigned>(n)) atomicMax(&words[t], static_cast<uint32_t>(i + 1) << LG_COUNT_BITS);
             }
-            __syncthreads();
+            if (n_bias) __syncthreads();   // the maximum is taken of whole words: no counts in them yet
+#pragma unroll 4
             for (int i = tid; i < n_hist; i += LG_THREADS) {
                 const unsigned t = static_cast<unsigned>(hist[i]) - static_cast<unsigned>(s0);
                 if (t < static_cast<unsigned>(n)) atomicAdd(&words[t], 1u);
             }
             __syncthreads();
         }
-        for (int i = tid; i < n; i += LG_THREADS) {
-            const int t = s0 + i;
-            float v = x[t];
-            if (n_hist || n_bias) {
-                const uint32_t w = words[i];
+#pragma unroll
+        for (int k = 0; k < LG_HELD / VEC; ++k) {
+            const int i = VEC * (k * LG_THREADS + tid);
+            if (i >= n) break;
+            uint32_t w[VEC] = {};
+            if (lists) {
+                if constexpr (VEC == 4)
+                    *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(words + i);
+                else
+                    w[0] = words[i];
+            }
+            const uint32_t bits = allow ? allow[(s0 + i) >> 5] >> ((s0 + i) & 31) : 0xffffffffu;   // VEC divides 32
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                if (w[e] || i + e >= n) continue;   // listed tokens: as they are for now
+                if (!(bits >> e & 1u)) v[VEC * k + e] = -INFINITY;
+                consider(v[VEC * k + e], s0 + i + e);
+            }
+            if (VEC == 4 && i + 3 < n)
+                *reinterpret_cast<float4*>(out + s0 + i) = *reinterpret_cast<const float4*>(v + VEC * k);
+            else
+                for (int e = 0; e < VEC; ++e)
+                    if (i + e < n) out[s0 + i + e] = v[VEC * k + e];
+        }
+        if (lists) {
+            __syncthreads();   // the logits of listed tokens stand in out
+            auto treat = [&](int token) {
+                const unsigned i = static_cast<unsigned>(token) - static_cast<unsigned>(s0);
+                const uint32_t w = i < static_cast<unsigned>(n) && words[i] ? atomicExch(&words[i], 0u) : 0u;
+                if (!w) return;
+                float y = out[token];
                 const uint32_t c = w & LG_MAX_HIST, b = w >> LG_COUNT_BITS;
                 if (c) {
-                    v = v > 0.0f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
-                    v = __fsub_rn(v, __fadd_rn(__fmul_rn(freq, static_cast<float>(c)), pres));
+                    y = y > 0.0f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
+                    y = __fsub_rn(y, __fadd_rn(__fmul_rn(freq, static_cast<float>(c)), pres));
                 }
-                if (b) v = __fadd_rn(v, p.bias[row * p.bias_stride + b - 1]);
-            }
-            if (allow && !(allow[t >> 5] >> (t & 31) & 1u)) v = -INFINITY;
-            out[t] = v;
-            if (v > best.v) best = Best{v, t};
+                if (b) y = __fadd_rn(y, p.bias[row * p.bias_stride + b - 1]);
+                if (!allowed(token)) y = -INFINITY;
+                out[token] = y;
+                consider(y, token);
+            };
+            for (int i = tid; i < n_hist; i += LG_THREADS) treat(hist[i]);
+            for (int i = tid; i < n_bias; i += LG_THREADS) treat(bias_token[i]);
+            __syncthreads();
         }
-        __syncthreads();
     }
     if (!p.argmax) return;   // the whole grid
     for (int o = 16; o >= 1; o >>= 1)
         take(best, Best{__shfl_xor_sync(0xffffffffu, best.v, o), __shfl_xor_sync(0xffffffffu, best.t, o)});
     if ((tid & 31) == 0) warp_best[tid >> 5] = best;
     __syncthreads();
-    if (tid == 0) {
+    if (tid == 0)
         for (int w = 1; w < LG_THREADS / 32; ++w) take(best, warp_best[w]);
-    }
     cluster.barrier_wait();   // every CTA of the row has started
-    if (tid == 0) {
-        *cluster.map_shared_rank(&cta_best[rank], 0) = best;
-    }
+    if (tid == 0) *cluster.map_shared_rank(&cta_best[rank], 0) = best;
     cluster.sync();
     if (rank == 0 && tid == 0) {
         for (int c = 1; c < LG_CLUSTER; ++c) take(best, cta_best[c]);
@@ -122,20 +174,26 @@ extern "C" mcpm_status mcpm_logits_process(const mcpm_logits_params* params, voi
     if (p.hist && (!p.penalties || p.hist_max < 0 || p.hist_max > LG_MAX_HIST || p.hist_stride < p.hist_max)) return MCPM_BAD_ARG;
     if (p.bias_token && (!p.bias || p.bias_max < 0 || p.bias_max > LG_MAX_BIAS || p.bias_stride < p.bias_max)) return MCPM_BAD_ARG;
     if (p.allow && p.allow_stride < mask_words) return MCPM_BAD_ARG;
-    cudaError_t e = cudaFuncSetAttribute(k_logits, cudaFuncAttributeMaxDynamicSharedMemorySize, LG_SLICE * 4);
+    auto aligned = [](const float* q, int64_t stride) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0 && stride % 4 == 0; };
+    void (*kernel)(mcpm_logits_params) =
+        aligned(p.logits, p.logits_stride) && aligned(p.out, p.out_stride) ? k_logits<4> : k_logits<1>;
+    const size_t smem = p.hist || p.bias_token ? LG_SLICE * 4 : 0;
+    cudaError_t e = smem ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LG_SLICE * 4) : cudaSuccess;
     if (e == cudaSuccess) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(static_cast<unsigned>(p.n_seq) * LG_CLUSTER);
         cfg.blockDim = dim3(LG_THREADS);
-        cfg.dynamicSmemBytes = p.hist || p.bias_token ? LG_SLICE * 4 : 0;
+        cfg.dynamicSmemBytes = smem;
         cfg.stream = static_cast<cudaStream_t>(stream);
-        cudaLaunchAttribute attr[1];
+        cudaLaunchAttribute attr[2];
         attr[0].id = cudaLaunchAttributeClusterDimension;
         attr[0].val.clusterDim.x = LG_CLUSTER;
         attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // every CTA waits before it reads
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        e = cudaLaunchKernelEx(&cfg, k_logits, p);
+        cfg.numAttrs = 2;
+        e = cudaLaunchKernelEx(&cfg, kernel, p);
     }
     if (e == cudaSuccess) return MCPM_OK;
     std::fprintf(stderr, "[mcpm] mcpm_logits_process: CUDA error: %s\n", cudaGetErrorString(e));

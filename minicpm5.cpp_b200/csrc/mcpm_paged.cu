@@ -1,7 +1,10 @@
 // Paged KV cache: append of new tokens (RoPE, rounding, page writes), attention of one new token
 // per sequence over its pages, and eviction of the positions with the least attention mass.
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
+
+#include <cooperative_groups.h>
 
 #include "../../include/mcpm.h"
 #include "mcpm_device.cuh"
@@ -16,39 +19,60 @@ struct AppendArgs {
     const int* table;
     void *kc, *vc;
     float* mass;
-    int n_seq, items;   // items: float4s of one token's q, k and v rows
+    int n_seq;
 };
 
-// One float4 (two rotary pairs) per thread; a token's items are its query heads, its KV heads' K,
-// then their V.  (x0, x1) -> (c x0 - s x1, s x0 + c x1), one fma per output as mcpm_rope_kv_append.
-template <typename T>
-__global__ void k_paged_append(const PagedGeom g, const AppendArgs a) {
+// A CTA per token; a token's rows are its query heads, its KV heads' K, then their V.  D / 4 lanes to a row, a
+// float4 (two rotary pairs, the same ones in every row) a lane, AP_HELD rows of a lane in flight.
+// (x0, x1) -> (c x0 - s x1, s x0 + c x1), one fma per output as mcpm_rope_kv_append.
+constexpr int AP_WARPS = 4, AP_HELD = 5;
+template <typename T, int D>
+__global__ void __launch_bounds__(32 * AP_WARPS) k_paged_append(const PagedGeom g, const AppendArgs a) {
+    constexpr int LANES = D / 4, AT_ONCE = AP_WARPS * 32 / LANES;   // lanes of a row, rows of the CTA
+    grid_dep_launch();
+    grid_dep_wait();
     const size_t i = blockIdx.x;
-    const int item = blockIdx.y * blockDim.x + threadIdx.x;
-    if (item >= a.items) return;
-    const int per_head = g.head_dim / 4, nq = a.t.q ? g.n_head * per_head : 0, nk = g.n_head_kv * per_head;
-    const int tok_slot = a.t.tok_slot[i];
-    const bool is_q = item < nq, is_v = item >= nq + nk;
-    const int x = is_q ? item : is_v ? item - nq - nk : item - nq;   // float4 within its row
-    const float* src = is_q ? a.t.q + i * a.t.q_stride : (is_v ? a.t.v : a.t.k) + i * a.t.kv_stride;
-    float4 v = reinterpret_cast<const float4*>(src)[x];
-    if (a.t.rope && !is_v) {
-        const int pos = min(max(a.t.tok_pos ? a.t.tok_pos[i] : tok_slot, 0), a.t.rope_len - 1);
-        const float4 cs = reinterpret_cast<const float4*>(a.t.rope)[static_cast<size_t>(pos) * per_head + x % per_head];
-        v = make_float4(__fmaf_rn(cs.x, v.x, -__fmul_rn(cs.y, v.y)), __fmaf_rn(cs.y, v.x, __fmul_rn(cs.x, v.y)),
-                        __fmaf_rn(cs.z, v.z, -__fmul_rn(cs.w, v.w)), __fmaf_rn(cs.w, v.z, __fmul_rn(cs.z, v.w)));
+    const int x = threadIdx.x % LANES, first = threadIdx.x / LANES, nq = a.t.q ? g.n_head : 0, nk = g.n_head_kv, rows = nq + 2 * nk;
+    const int tok_slot = a.t.tok_slot[i], seq = a.t.tok_seq ? a.t.tok_seq[i] : static_cast<int>(i);
+    const int pos = a.t.tok_pos ? a.t.tok_pos[i] : tok_slot;
+    const float4 cs = a.t.rope ? reinterpret_cast<const float4*>(a.t.rope)[static_cast<size_t>(min(max(pos, 0), a.t.rope_len - 1)) * LANES + x]
+                               : make_float4(1.0f, 0.0f, 1.0f, 0.0f);
+    int page = -1, slot = 0;
+    const bool held = seq >= 0 && seq < a.n_seq && tok_slot >= 0 && tok_slot < g.max_pages * g.page_size &&
+                      g.locate(a.table + static_cast<size_t>(seq) * g.max_pages, tok_slot, page, slot);
+    for (int r0 = first; r0 < rows; r0 += AT_ONCE * AP_HELD) {
+        float4 v[AP_HELD];
+#pragma unroll
+        for (int k = 0; k < AP_HELD; ++k) {
+            const int r = r0 + k * AT_ONCE;
+            if (r >= rows) break;
+            const float* src = r < nq ? a.t.q + i * a.t.q_stride + r * D
+                                      : (r < nq + nk ? a.t.k : a.t.v) + i * a.t.kv_stride + (r < nq + nk ? r - nq : r - nq - nk) * D;
+            v[k] = reinterpret_cast<const float4*>(src)[x];
+        }
+#pragma unroll
+        for (int k = 0; k < AP_HELD; ++k) {
+            const int r = r0 + k * AT_ONCE;
+            if (r >= rows) break;
+            float4 y = v[k];
+            if (a.t.rope && r < nq + nk)
+                y = make_float4(__fmaf_rn(cs.x, y.x, -__fmul_rn(cs.y, y.y)), __fmaf_rn(cs.y, y.x, __fmul_rn(cs.x, y.y)),
+                                __fmaf_rn(cs.z, y.z, -__fmul_rn(cs.w, y.w)), __fmaf_rn(cs.w, y.z, __fmul_rn(cs.z, y.w)));
+            if (r < nq) {
+                reinterpret_cast<float4*>(a.t.q_out + (i * g.n_head + r) * D)[x] = y;
+            } else if (held) {
+                const bool is_v = r >= nq + nk;
+                const int head = r - nq - (is_v ? nk : 0);
+                kv_store4(static_cast<T*>(is_v ? a.vc : a.kc) + g.row(page, slot, head) + 4 * x, y);
+                if (!is_v && x == 0 && a.mass) a.mass[g.mass_at(page, slot, head)] = 0.0f;
+            }
+        }
     }
-    if (is_q) {
-        reinterpret_cast<float4*>(a.t.q_out + i * g.n_head * g.head_dim)[x] = v;
-        return;
-    }
-    const int seq = a.t.tok_seq ? a.t.tok_seq[i] : static_cast<int>(i);
-    if (seq < 0 || seq >= a.n_seq || tok_slot < 0 || tok_slot >= g.max_pages * g.page_size) return;
-    int page, slot;
-    if (!g.locate(a.table + static_cast<size_t>(seq) * g.max_pages, tok_slot, page, slot)) return;
-    const int head = x / per_head;
-    kv_store4(static_cast<T*>(is_v ? a.vc : a.kc) + g.row(page, slot, head) + 4 * (x % per_head), v);
-    if (!is_v && x % per_head == 0 && a.mass) a.mass[g.mass_at(page, slot, head)] = 0.0f;
+}
+
+template <typename T>
+cudaError_t launch_append(const PagedGeom& g, const AppendArgs& a, cudaStream_t s) {
+    return launch_dependent(g.head_dim == 64 ? k_paged_append<T, 64> : k_paged_append<T, 128>, dim3(a.t.n_tok), 32 * AP_WARPS, 0, s, g, a);
 }
 
 // ---------------------------------------------------------------- eviction
@@ -60,107 +84,229 @@ struct EvictArgs {
     int n_keep, n_sink, n_recent;
 };
 
-constexpr int EV_THREADS = 1024;
+constexpr int EV_THREADS = 1024, EV_WARPS = EV_THREADS / 32;
+constexpr int EV_MAX_CLUSTER = 8;
+constexpr int EV_BITS = 11, EV_BINS = 1 << EV_BITS, EV_PASSES = 3;   // digits of 11, 11 and 10 bits, highest first
+constexpr int EV_KEYS = 32768;                                       // keys a CTA holds in shared memory
+constexpr int EV_SMEM = (EV_PASSES * EV_BINS + EV_KEYS) * 4;
 
-// Order-preserving unsigned key of a position: a larger key is kept first.  NaN 0 (lightest), then the
-// floats in order (-0 and +0 alike), then the protected positions.
+// Order-preserving unsigned key of a position: a larger key is kept first.  Absent positions 0, NaN 1
+// (lightest), then the floats in order (-0 and +0 alike), then the protected positions.
 __device__ __forceinline__ uint32_t mass_key(float m) {
-    if (m != m) return 0u;
+    if (m != m) return 1u;
     const uint32_t u = __float_as_uint(m + 0.0f);
-    return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+    return (u & 0x80000000u) ? ~u : u | 0x80000000u;   // -inf is 0x007fffff
 }
 
-// One CTA per (KV head, sequence): radix selection of the n_keep-th largest key, 8 bits a pass, then
-// the kept positions in order.
+// A cluster per (KV head, sequence), each CTA with a contiguous share of the positions.  Radix selection of
+// the n_keep-th largest key: per digit a histogram in each CTA, summed over the cluster, and the bin in
+// which the count from above reaches n_keep.  Then every warp counts its positions above and at the
+// threshold, and writes its part of the list in order.  Keys stay in shared memory between the passes.
 __global__ void __launch_bounds__(EV_THREADS, 1) k_paged_evict_select(const PagedGeom g, const EvictArgs a) {
-    __shared__ int hist[256], warp_gt[32], warp_eq[32], pick[2];
-    const int kv = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    extern __shared__ __align__(16) uint32_t ev_smem[];
+    __shared__ int warp_sum[EV_WARPS], warp_gt[EV_WARPS], warp_eq[EV_WARPS], cta_gt, cta_eq, pick[3];
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    grid_dep_launch();
+    grid_dep_wait();
+    uint32_t* hist = ev_smem;   // [EV_PASSES][EV_BINS]
+    uint32_t* keys = ev_smem + EV_PASSES * EV_BINS;
+    const int n_cta = cluster.num_blocks(), rank = cluster.block_rank();
+    const int kv = blockIdx.x / n_cta, seq = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int n = g.clamp_len(a.len[seq]);
+    const int share = ((n + n_cta - 1) / n_cta + 31) & ~31;
+    const int lo = min(n, rank * share), m = min(n, lo + share) - lo;   // this CTA's positions lo .. lo + m - 1
     const int* row = a.table + static_cast<size_t>(seq) * g.max_pages;
     int* kept = a.kept + (static_cast<size_t>(seq) * g.n_head_kv + kv) * a.n_keep;
-    auto key_of = [&](int j, bool& present) -> uint32_t {
+    auto read_key = [&](int i) -> uint32_t {
+        const int j = lo + i;
         int page, slot;
-        present = g.locate(row, j, page, slot);
-        if (!present) return 0u;
+        if (!g.locate(row, j, page, slot)) return 0u;
         if (j < a.n_sink || j >= n - a.n_recent) return 0xffffffffu;
         return mass_key(a.mass[g.mass_at(page, slot, kv)]);
     };
-    // threshold key and how many positions with exactly that key are kept; a length within the budget
-    // keeps every present position (threshold 0, no limit)
+    auto key = [&](int i) { return i < EV_KEYS ? keys[i] : read_key(i); };
+    for (int i = tid; i < EV_PASSES * EV_BINS; i += EV_THREADS) hist[i] = 0u;
+    __syncthreads();
+    for (int i = tid; i < m; i += EV_THREADS) {
+        const uint32_t k = read_key(i);
+        if (i < EV_KEYS) keys[i] = k;
+        if (k) atomicAdd(&hist[k >> (32 - EV_BITS)], 1u);
+    }
+    // Threshold key and how many positions with exactly that key are kept.  Fewer present positions than
+    // n_keep: the scans end in bin 0 with room to spare, the threshold is 0, which absent positions alone have.
     uint32_t prefix = 0u;
-    int need = a.n_keep, total = 0;
-    for (int sh = 24; sh >= 0; sh -= 8) {
-        for (int i = tid; i < 256; i += EV_THREADS) hist[i] = 0;
+    int need = a.n_keep;
+    for (int pass = 0; pass < EV_PASSES; ++pass) {
+        const int low = pass == 0 ? 32 - EV_BITS : pass == 1 ? 32 - 2 * EV_BITS : 0;   // lowest bit of the digit
+        uint32_t* mine = hist + pass * EV_BINS;
+        if (pass > 0) {
+            const int above = low + (pass == 1 ? EV_BITS : 32 - 2 * EV_BITS);
+            for (int i = tid; i < m; i += EV_THREADS) {
+                const uint32_t k = key(i);
+                if (k && (k >> above) == (prefix >> above)) atomicAdd(&mine[(k >> low) & (EV_BINS - 1) & ((1u << (above - low)) - 1u)], 1u);
+            }
+        }
+        if (n_cta > 1)
+            cluster.sync();
+        else
+            __syncthreads();
+        // two bins a thread, highest bins first: bins b and b - 1
+        const int b = EV_BINS - 1 - 2 * tid;
+        int c0 = 0, c1 = 0;
+        for (int r = 0; r < n_cta; ++r) {
+            const uint32_t* h = n_cta > 1 ? cluster.map_shared_rank(mine, r) : mine;
+            c0 += h[b];
+            c1 += h[b - 1];
+        }
+        int x = c0 + c1;   // inclusive scan over the threads
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) warp_sum[warp] = x;
         __syncthreads();
-        for (int j = tid; j < n; j += EV_THREADS) {
-            bool present;
-            const uint32_t k = key_of(j, present);
-            if (present && (sh == 24 || (k >> (sh + 8)) == (prefix >> (sh + 8)))) atomicAdd(&hist[(k >> sh) & 255], 1);
+        int w = warp_sum[lane];
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, w, o);
+            if (lane >= o) w += y;
+        }
+        const int all = __shfl_sync(0xffffffffu, w, 31), before_warp = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
+        const int before = x - c0 - c1 + (warp ? before_warp : 0);   // positions in higher bins
+        if (before < need && before + c0 + c1 >= need) {
+            const bool first = before + c0 >= need;
+            pick[0] = first ? b : b - 1;
+            pick[1] = first ? before : before + c0;
+        } else if (tid == EV_THREADS - 1 && all < need) {   // bin 0 is taken whole
+            pick[0] = 0;
+            pick[1] = all - c1;
         }
         __syncthreads();
-        if (tid == 0) {
-            int above = 0, b = 255;
-            for (; b > 0 && above + hist[b] < need; --b) above += hist[b];
-            pick[0] = b;
-            pick[1] = above;
-            if (sh == 24)
-                for (int i = 0; i < 256; ++i) total += hist[i];
-        }
-        __syncthreads();
-        prefix |= static_cast<uint32_t>(pick[0]) << sh;
+        prefix |= static_cast<uint32_t>(pick[0]) << low;
         need -= pick[1];
         __syncthreads();
     }
-    if (tid == 0) pick[0] = total;
-    __syncthreads();
-    total = pick[0];
-    int at = 0, eq_seen = 0;   // kept so far, threshold-equal positions seen so far
-    for (int j0 = 0; j0 < n; j0 += EV_THREADS) {
-        const int j = j0 + tid;
-        bool present = false;
-        const uint32_t k = j < n ? key_of(j, present) : 0u;
-        const bool gt = present && k > prefix, eq = present && k == prefix;
-        const unsigned mg = __ballot_sync(0xffffffffu, gt), me = __ballot_sync(0xffffffffu, eq);
-        if (lane == 0) warp_gt[warp] = __popc(mg), warp_eq[warp] = __popc(me);
-        __syncthreads();
-        int gt_before = 0, eq_before = 0, gt_all = 0, eq_all = 0;
-        for (int w = 0; w < 32; ++w) {
-            if (w < warp) gt_before += warp_gt[w], eq_before += warp_eq[w];
-            gt_all += warp_gt[w], eq_all += warp_eq[w];
-        }
-        const unsigned below = (1u << lane) - 1u;
-        gt_before += __popc(mg & below);
-        eq_before += __popc(me & below);
-        const int eq_rank = eq_seen + eq_before;
-        const int place = at + gt_before + (min(eq_rank, need) - min(eq_seen, need));
-        if (gt || (eq && eq_rank < need)) kept[place] = j;
-        at += gt_all + min(eq_seen + eq_all, need) - min(eq_seen, need);
-        eq_seen += eq_all;
-        __syncthreads();
+    // each warp's contiguous positions: how many are above the threshold, how many at it
+    const int per = ((m + EV_WARPS - 1) / EV_WARPS + 31) & ~31;
+    const int w0 = min(m, warp * per), w1 = min(m, w0 + per);
+    int gt = 0, eq = 0;
+    for (int i = w0 + lane; i - lane < w1; i += 32) {
+        const uint32_t k = i < w1 ? key(i) : 0u;
+        gt += __popc(__ballot_sync(0xffffffffu, k > prefix));
+        eq += __popc(__ballot_sync(0xffffffffu, k && k == prefix));
     }
-    for (int i = at + tid; i < a.n_keep; i += EV_THREADS) kept[i] = -1;
-    if (tid == 0 && kv == 0) a.new_len[seq] = at;
+    if (lane == 0) warp_gt[warp] = gt, warp_eq[warp] = eq;
+    __syncthreads();
+    int g0 = 0, e0 = 0;   // before this warp
+    for (int w = 0; w < EV_WARPS; ++w) {
+        if (w == warp && tid != 0) break;
+        if (w < warp) g0 += warp_gt[w], e0 += warp_eq[w];
+        if (tid == 0) cta_gt = (w ? cta_gt : 0) + warp_gt[w], cta_eq = (w ? cta_eq : 0) + warp_eq[w];
+    }
+    int g_all = 0, e_all = 0;
+    if (n_cta > 1) {
+        cluster.sync();
+        for (int r = 0; r < n_cta; ++r) {
+            const int cg_ = *cluster.map_shared_rank(&cta_gt, r), ce = *cluster.map_shared_rank(&cta_eq, r);
+            if (r < rank) g0 += cg_, e0 += ce;
+            g_all += cg_, e_all += ce;
+        }
+    } else {
+        __syncthreads();
+        g_all = cta_gt, e_all = cta_eq;
+    }
+    for (int i = w0 + lane; i - lane < w1; i += 32) {
+        const uint32_t k = i < w1 ? key(i) : 0u;
+        const bool above = k > prefix, at = k && k == prefix;
+        const unsigned mg = __ballot_sync(0xffffffffu, above), me = __ballot_sync(0xffffffffu, at), below = (1u << lane) - 1u;
+        const int eq_rank = e0 + __popc(me & below);
+        if (above || (at && eq_rank < need)) kept[g0 + __popc(mg & below) + min(eq_rank, need)] = lo + i;
+        g0 += __popc(mg);
+        e0 += __popc(me);
+    }
+    const int total = g_all + min(e_all, need);
+    for (int i = total + rank * EV_THREADS + tid; i < a.n_keep; i += n_cta * EV_THREADS) kept[i] = -1;
+    if (tid == 0 && kv == 0 && rank == 0) a.new_len[seq] = total;
+    if (n_cta > 1) cluster.sync();   // no CTA ends while another reads its counts
 }
 
-// A warp per kept row: K, V (16 bytes a lane) and the mass.
-template <typename T>
-__global__ void k_paged_evict_copy(const PagedGeom g, const EvictArgs a) {
-    const int i = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5), kv = blockIdx.y, seq = blockIdx.z;
-    const int lane = threadIdx.x & 31;
-    if (i >= a.n_keep) return;
-    const int j = a.kept[(static_cast<size_t>(seq) * g.n_head_kv + kv) * a.n_keep + i];
-    if (j < 0) return;
-    int sp, ss, dp, ds;
-    if (!g.locate(a.table + static_cast<size_t>(seq) * g.max_pages, j, sp, ss)) return;
-    if (!g.locate(a.dst + static_cast<size_t>(seq) * g.max_pages, i, dp, ds)) return;
-    const long long so = g.row(sp, ss, kv), to = g.row(dp, ds, kv);
-    T *kc = static_cast<T*>(a.kc), *vc = static_cast<T*>(a.vc);
-    const int chunks = g.head_dim * static_cast<int>(sizeof(T)) / 16;
-    for (int c = lane; c < chunks; c += 32) {
-        reinterpret_cast<uint4*>(kc + to)[c] = reinterpret_cast<const uint4*>(kc + so)[c];
-        reinterpret_cast<uint4*>(vc + to)[c] = reinterpret_cast<const uint4*>(vc + so)[c];
+// A warp per EV_ROWS kept rows: K, V (16 bytes a lane, eight loads in flight) and the mass.
+constexpr int EV_ROWS = 8, EV_COPY_WARPS = 4;
+template <typename T, int D>
+__global__ void __launch_bounds__(32 * EV_COPY_WARPS) k_paged_evict_copy(const PagedGeom g, const EvictArgs a) {
+    constexpr int CH = D * static_cast<int>(sizeof(T)) / 16, ITEMS = EV_ROWS * 2 * CH / 32;   // chunks of a row; 16-byte copies a lane
+    grid_dep_launch();
+    grid_dep_wait();
+    const int i0 = (blockIdx.x * EV_COPY_WARPS + (threadIdx.x >> 5)) * EV_ROWS, kv = blockIdx.y, seq = blockIdx.z;
+    const int lane = threadIdx.x & 31, i = i0 + lane;
+    if (i0 >= a.n_keep) return;
+    long long from = -1, to = -1;
+    if (lane < EV_ROWS && i < a.n_keep) {
+        const int j = a.kept[(static_cast<size_t>(seq) * g.n_head_kv + kv) * a.n_keep + i];
+        int sp, ss, dp, ds;
+        const bool dst = g.locate(a.dst + static_cast<size_t>(seq) * g.max_pages, i, dp, ds);
+        if (j >= 0 && dst && g.locate(a.table + static_cast<size_t>(seq) * g.max_pages, j, sp, ss)) {
+            from = g.row(sp, ss, kv);
+            to = g.row(dp, ds, kv);
+            a.mass[g.mass_at(dp, ds, kv)] = a.mass[g.mass_at(sp, ss, kv)];
+        }
     }
-    if (lane == 0) a.mass[g.mass_at(dp, ds, kv)] = a.mass[g.mass_at(sp, ss, kv)];
+    T *kc = static_cast<T*>(a.kc), *vc = static_cast<T*>(a.vc);
+#pragma unroll
+    for (int b = 0; b < ITEMS; b += 8) {
+        uint4 x[8];
+#pragma unroll
+        for (int k = 0; k < 8 && b + k < ITEMS; ++k) {
+            const int at = (b + k) * 32 + lane, r = at / (2 * CH), c = at % (2 * CH);
+            const long long o = __shfl_sync(0xffffffffu, from, r);
+            if (o >= 0) x[k] = __ldcs(reinterpret_cast<const uint4*>((c < CH ? kc : vc) + o) + c % CH);
+        }
+#pragma unroll
+        for (int k = 0; k < 8 && b + k < ITEMS; ++k) {
+            const int at = (b + k) * 32 + lane, r = at / (2 * CH), c = at % (2 * CH);
+            const long long o = __shfl_sync(0xffffffffu, to, r);
+            if (o >= 0) reinterpret_cast<uint4*>((c < CH ? kc : vc) + o)[c % CH] = x[k];
+        }
+    }
+}
+
+template <typename T>
+cudaError_t launch_evict_copy(const PagedGeom& g, const EvictArgs& a, int n_seq, cudaStream_t s) {
+    const int per = EV_ROWS * EV_COPY_WARPS;
+    const dim3 grid((a.n_keep + per - 1) / per, g.n_head_kv, n_seq);
+    return launch_dependent(g.head_dim == 64 ? k_paged_evict_copy<T, 64> : k_paged_evict_copy<T, 128>, grid, 32 * EV_COPY_WARPS, 0, s, g, a);
+}
+
+// One CTA for up to 4096 positions, more where the table has room for longer sequences and SMs are free.
+cudaError_t launch_evict_select(const PagedGeom& g, const EvictArgs& a, int n_seq, cudaStream_t s) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    static bool prepared[64] = {};
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!prepared[dev]) {
+        e = cudaFuncSetAttribute(k_paged_evict_select, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_SMEM);
+        if (e != cudaSuccess) return e;
+        prepared[dev] = true;
+    }
+    const long long room = static_cast<long long>(g.max_pages) * g.page_size, pairs = static_cast<long long>(n_seq) * g.n_head_kv;
+    int cluster = 1;
+    while (cluster < EV_MAX_CLUSTER && cluster * 4096LL < room && pairs * cluster * 2 <= 148) cluster *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(g.n_head_kv * cluster, n_seq);
+    cfg.blockDim = dim3(EV_THREADS);
+    const long long keys = std::min<long long>(EV_KEYS, (room + cluster - 1) / cluster + 32);
+    cfg.dynamicSmemBytes = (EV_PASSES * EV_BINS + static_cast<size_t>(keys)) * 4;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, k_paged_evict_select, g, a);
 }
 
 // ---------------------------------------------------------------- host side
@@ -245,7 +391,7 @@ mcpm_status mcpm_paged_append(const mcpm_paged_config* cfg, const mcpm_paged_poo
     if (st == MCPM_OK) st = check_pool(pool);
     if (st != MCPM_OK) return st;
     if (!tokens || !table || n_seq <= 0 || n_seq > cfg->max_seqs) return MCPM_BAD_ARG;
-    AppendArgs a{*tokens, table, pool->k, pool->v, pool->mass, n_seq, 0};
+    AppendArgs a{*tokens, table, pool->k, pool->v, pool->mass, n_seq};
     mcpm_paged_tokens& t = a.t;
     const int q_row = g.n_head * g.head_dim, kv_row = g.n_head_kv * g.head_dim;
     if (t.q_stride == 0) t.q_stride = q_row;
@@ -258,16 +404,10 @@ mcpm_status mcpm_paged_append(const mcpm_paged_config* cfg, const mcpm_paged_poo
         return MCPM_BAD_ARG;
     if (t.rope && (t.rope_len <= 0 || !aligned16(t.rope))) return MCPM_BAD_ARG;
     if (t.n_tok == 0) return MCPM_OK;
-    a.items = ((t.q ? g.n_head : 0) + 2 * g.n_head_kv) * g.head_dim / 4;
-    const dim3 grid(t.n_tok, (a.items + 127) / 128);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (cfg->kv_type == MCPM_KV_F32)
-        k_paged_append<float><<<grid, 128, 0, s>>>(g, a);
-    else if (cfg->kv_type == MCPM_KV_F16)
-        k_paged_append<__half><<<grid, 128, 0, s>>>(g, a);
-    else
-        k_paged_append<__nv_bfloat16><<<grid, 128, 0, s>>>(g, a);
-    return status("mcpm_paged_append", cudaGetLastError());
+    return status("mcpm_paged_append", cfg->kv_type == MCPM_KV_F32   ? launch_append<float>(g, a, s)
+                                       : cfg->kv_type == MCPM_KV_F16 ? launch_append<__half>(g, a, s)
+                                                                     : launch_append<__nv_bfloat16>(g, a, s));
 }
 
 mcpm_status mcpm_paged_attention(const mcpm_paged_config* cfg, const mcpm_paged_pool* pool, const int* table,
@@ -301,15 +441,12 @@ mcpm_status mcpm_paged_evict(const mcpm_paged_config* cfg, const mcpm_paged_pool
         return MCPM_BAD_ARG;
     EvictArgs a{pool->k, pool->v, pool->mass, table, seq_len, dst_table, new_len, kept, n_keep, n_sink, n_recent};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    k_paged_evict_select<<<dim3(g.n_head_kv, n_seq), EV_THREADS, 0, s>>>(g, a);
-    const dim3 grid((n_keep + 3) / 4, g.n_head_kv, n_seq);
-    if (cfg->kv_type == MCPM_KV_F32)
-        k_paged_evict_copy<float><<<grid, 128, 0, s>>>(g, a);
-    else if (cfg->kv_type == MCPM_KV_F16)
-        k_paged_evict_copy<__half><<<grid, 128, 0, s>>>(g, a);
-    else
-        k_paged_evict_copy<__nv_bfloat16><<<grid, 128, 0, s>>>(g, a);
-    return status("mcpm_paged_evict", cudaGetLastError());
+    cudaError_t e = launch_evict_select(g, a, n_seq, s);
+    if (e == cudaSuccess)
+        e = cfg->kv_type == MCPM_KV_F32   ? launch_evict_copy<float>(g, a, n_seq, s)
+            : cfg->kv_type == MCPM_KV_F16 ? launch_evict_copy<__half>(g, a, n_seq, s)
+                                          : launch_evict_copy<__nv_bfloat16>(g, a, n_seq, s);
+    return status("mcpm_paged_evict", e);
 }
 
 }  // extern "C"
