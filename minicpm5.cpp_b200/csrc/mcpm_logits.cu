@@ -13,8 +13,11 @@ namespace {
 
 constexpr int LG_CLUSTER = 8;        // CTAs that share a row
 constexpr int LG_THREADS = 512;
-constexpr int LG_HELD = 32;          // logits a thread holds at once
-constexpr int LG_SLICE = LG_THREADS * LG_HELD;   // tokens whose counters a CTA holds at once (one word each)
+constexpr int LG_HELD = 8;           // logits a thread holds at once: 40 registers, three CTAs per SM
+constexpr int LG_STEP = LG_THREADS * LG_HELD;
+constexpr int LG_SLICE = 4 * LG_STEP;   // tokens whose counters a CTA holds at once (one word each)
+constexpr int LG_LIST = 1024;        // listed tokens that are put aside at once
+constexpr int LG_BATCH = 4;          // list entries of a thread in flight
 constexpr int LG_COUNT_BITS = 20;    // counter word: times in the history; above: last bias entry + 1
 constexpr int LG_MAX_HIST = (1 << LG_COUNT_BITS) - 1, LG_MAX_BIAS = (1 << (32 - LG_COUNT_BITS)) - 2;
 
@@ -28,14 +31,18 @@ __device__ __forceinline__ void take(Best& a, const Best& b) {
 }
 
 // A cluster of LG_CLUSTER CTAs per row, each with a contiguous share of the vocabulary, LG_SLICE tokens at a
-// time.  The slice's logits are on their way to registers while the history is counted into shared-memory
-// words (integer atomics: the order does not matter) and each bias entry leaves its index there (the largest,
-// hence the last entry, stays).  Tokens without a word go through at once, only masked.  The others are few:
-// the lists are walked again, and whoever takes a token's word first treats it, so no warp of the streaming
-// pass waits for one lane's division.  VEC = 4 where all rows are 16-byte aligned, else 1.
+// time.  The slice's first logits are on their way to registers while the history is counted into
+// shared-memory words (integer atomics: the order does not matter) and each bias entry leaves its index there
+// (the largest, hence the last entry, stays).  Tokens without a word go through at once, only masked.  The
+// others are few and would hold every warp up with their division, so they are put aside and treated together
+// afterwards (beyond LG_LIST of them in a slice, on the spot).  VEC = 4 where all rows are 16-byte aligned,
+// else 1.
 template <int VEC>
-__global__ void __launch_bounds__(LG_THREADS, 2) k_logits(const mcpm_logits_params p) {
-    extern __shared__ __align__(16) uint32_t words[];
+__global__ void __launch_bounds__(LG_THREADS, 3) k_logits(const mcpm_logits_params p) {
+    extern __shared__ __align__(16) uint32_t words[];   // [LG_SLICE]
+    __shared__ float aside_v[LG_LIST];
+    __shared__ uint32_t aside_t[LG_LIST];   // token - s0, bit 31: allowed
+    __shared__ int n_aside;
     __shared__ Best warp_best[LG_THREADS / 32], cta_best[LG_CLUSTER];
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
@@ -59,24 +66,37 @@ __global__ void __launch_bounds__(LG_THREADS, 2) k_logits(const mcpm_logits_para
     auto consider = [&](float v, int t) {   // the lowest token of the largest value, whatever the order of calls
         if (v > best.v || (v == best.v && t < best.t && v > -INFINITY)) best = Best{v, t};
     };
-    auto allowed = [&](int t) { return !allow || (allow[t >> 5] >> (t & 31) & 1u); };
+    auto listed = [&](float y, uint32_t w, bool ok) {
+        const uint32_t c = w & LG_MAX_HIST, b = w >> LG_COUNT_BITS;
+        if (c) {
+            y = y > 0.0f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
+            y = __fsub_rn(y, __fadd_rn(__fmul_rn(freq, static_cast<float>(c)), pres));
+        }
+        if (b) y = __fadd_rn(y, p.bias[row * p.bias_stride + b - 1]);
+        return ok ? y : -INFINITY;
+    };
     for (int s0 = lo; s0 < hi; s0 += LG_SLICE) {
         const int n = min(LG_SLICE, hi - s0);
         float v[LG_HELD];
-        if constexpr (VEC == 4) {
+        uint32_t bits[LG_HELD / VEC];   // VEC divides 32: a load's tokens share a mask word
+        auto load = [&](int c) {
 #pragma unroll
-            for (int k = 0; k < LG_HELD / 4; ++k) {
-                const int i = 4 * (k * LG_THREADS + tid);
-                if (i + 3 < n)
-                    *reinterpret_cast<float4*>(v + 4 * k) = *reinterpret_cast<const float4*>(x + s0 + i);
+            for (int k = 0; k < LG_HELD / VEC; ++k) {
+                const int i = c + VEC * (k * LG_THREADS + tid);
+                if (VEC == 4 && i + 3 < n)
+                    *reinterpret_cast<float4*>(v + VEC * k) = *reinterpret_cast<const float4*>(x + s0 + i);
                 else
-                    for (int e = 0; e < 4; ++e) v[4 * k + e] = i + e < n ? x[s0 + i + e] : 0.0f;
+                    for (int e = 0; e < VEC; ++e) v[VEC * k + e] = i + e < n ? x[s0 + i + e] : 0.0f;
             }
-        } else {
 #pragma unroll
-            for (int k = 0; k < LG_HELD; ++k) v[k] = k * LG_THREADS + tid < n ? x[s0 + k * LG_THREADS + tid] : 0.0f;
-        }
+            for (int k = 0; k < LG_HELD / VEC; ++k) {
+                const int i = c + VEC * (k * LG_THREADS + tid);
+                bits[k] = allow && i < n ? allow[(s0 + i) >> 5] >> ((s0 + i) & 31) : 0xffffffffu;
+            }
+        };
+        load(0);
         if (lists) {
+            if (tid == 0) n_aside = 0;
             for (int i = tid; i < (n + 3) / 4; i += LG_THREADS) reinterpret_cast<uint4*>(words)[i] = make_uint4(0u, 0u, 0u, 0u);
             __syncthreads();
             for (int i = tid; i < n_bias; i += LG_THREADS) {
@@ -84,56 +104,63 @@ __global__ void __launch_bounds__(LG_THREADS, 2) k_logits(const mcpm_logits_para
                 if (t < static_cast<unsigned>(n)) atomicMax(&words[t], static_cast<uint32_t>(i + 1) << LG_COUNT_BITS);
             }
             if (n_bias) __syncthreads();   // the maximum is taken of whole words: no counts in them yet
-#pragma unroll 4
-            for (int i = tid; i < n_hist; i += LG_THREADS) {
-                const unsigned t = static_cast<unsigned>(hist[i]) - static_cast<unsigned>(s0);
-                if (t < static_cast<unsigned>(n)) atomicAdd(&words[t], 1u);
+            for (int i0 = tid; i0 < n_hist; i0 += LG_BATCH * LG_THREADS) {
+                unsigned t[LG_BATCH];
+#pragma unroll
+                for (int k = 0; k < LG_BATCH; ++k)
+                    t[k] = i0 + k * LG_THREADS < n_hist ? static_cast<unsigned>(hist[i0 + k * LG_THREADS]) - static_cast<unsigned>(s0) : ~0u;
+#pragma unroll
+                for (int k = 0; k < LG_BATCH; ++k)
+                    if (t[k] < static_cast<unsigned>(n)) atomicAdd(&words[t[k]], 1u);
             }
             __syncthreads();
         }
+        for (int c = 0; c < n; c += LG_STEP) {
+            if (c) load(c);
 #pragma unroll
-        for (int k = 0; k < LG_HELD / VEC; ++k) {
-            const int i = VEC * (k * LG_THREADS + tid);
-            if (i >= n) break;
-            uint32_t w[VEC] = {};
-            if (lists) {
-                if constexpr (VEC == 4)
-                    *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(words + i);
+            for (int k = 0; k < LG_HELD / VEC; ++k) {
+                const int i = c + VEC * (k * LG_THREADS + tid);
+                if (i >= n) break;
+                uint32_t w[VEC] = {};
+                if (lists) {
+                    if constexpr (VEC == 4)
+                        *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(words + i);
+                    else
+                        w[0] = words[i];
+                }
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const bool ok = bits[k] >> e & 1u;
+                    float& y = v[VEC * k + e];
+                    if (i + e >= n) continue;
+                    if (w[e]) {
+                        const int at = atomicAdd(&n_aside, 1);
+                        if (at < LG_LIST) {
+                            aside_v[at] = y;
+                            aside_t[at] = static_cast<uint32_t>(i + e) | static_cast<uint32_t>(ok) << 31;
+                            continue;   // its place in out is written again below
+                        }
+                        y = listed(y, w[e], ok);
+                    } else if (!ok) {
+                        y = -INFINITY;
+                    }
+                    if (y > best.v) best = Best{y, s0 + i + e};   // tokens ascend here
+                }
+                if (VEC == 4 && i + 3 < n)
+                    *reinterpret_cast<float4*>(out + s0 + i) = *reinterpret_cast<const float4*>(v + VEC * k);
                 else
-                    w[0] = words[i];
+                    for (int e = 0; e < VEC; ++e)
+                        if (i + e < n) out[s0 + i + e] = v[VEC * k + e];
             }
-            const uint32_t bits = allow ? allow[(s0 + i) >> 5] >> ((s0 + i) & 31) : 0xffffffffu;   // VEC divides 32
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                if (w[e] || i + e >= n) continue;   // listed tokens: as they are for now
-                if (!(bits >> e & 1u)) v[VEC * k + e] = -INFINITY;
-                consider(v[VEC * k + e], s0 + i + e);
-            }
-            if (VEC == 4 && i + 3 < n)
-                *reinterpret_cast<float4*>(out + s0 + i) = *reinterpret_cast<const float4*>(v + VEC * k);
-            else
-                for (int e = 0; e < VEC; ++e)
-                    if (i + e < n) out[s0 + i + e] = v[VEC * k + e];
         }
         if (lists) {
-            __syncthreads();   // the logits of listed tokens stand in out
-            auto treat = [&](int token) {
-                const unsigned i = static_cast<unsigned>(token) - static_cast<unsigned>(s0);
-                const uint32_t w = i < static_cast<unsigned>(n) && words[i] ? atomicExch(&words[i], 0u) : 0u;
-                if (!w) return;
-                float y = out[token];
-                const uint32_t c = w & LG_MAX_HIST, b = w >> LG_COUNT_BITS;
-                if (c) {
-                    y = y > 0.0f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
-                    y = __fsub_rn(y, __fadd_rn(__fmul_rn(freq, static_cast<float>(c)), pres));
-                }
-                if (b) y = __fadd_rn(y, p.bias[row * p.bias_stride + b - 1]);
-                if (!allowed(token)) y = -INFINITY;
-                out[token] = y;
-                consider(y, token);
-            };
-            for (int i = tid; i < n_hist; i += LG_THREADS) treat(hist[i]);
-            for (int i = tid; i < n_bias; i += LG_THREADS) treat(bias_token[i]);
+            __syncthreads();
+            for (int k = tid; k < min(n_aside, LG_LIST); k += LG_THREADS) {
+                const int i = static_cast<int>(aside_t[k] & 0x7fffffffu);
+                const float y = listed(aside_v[k], words[i], aside_t[k] >> 31);
+                out[s0 + i] = y;
+                consider(y, s0 + i);
+            }
             __syncthreads();
         }
     }

@@ -87,7 +87,8 @@ struct EvictArgs {
 constexpr int EV_THREADS = 1024, EV_WARPS = EV_THREADS / 32;
 constexpr int EV_MAX_CLUSTER = 8;
 constexpr int EV_BITS = 11, EV_BINS = 1 << EV_BITS, EV_PASSES = 3;   // digits of 11, 11 and 10 bits, highest first
-constexpr int EV_KEYS = 32768;                                       // keys a CTA holds in shared memory
+constexpr int EV_KEYS = 32768;   // keys a CTA holds in shared memory
+constexpr int EV_HELD = 4;       // positions a thread reads at once
 constexpr int EV_SMEM = (EV_PASSES * EV_BINS + EV_KEYS) * 4;
 
 // Order-preserving unsigned key of a position: a larger key is kept first.  Absent positions 0, NaN 1
@@ -104,7 +105,8 @@ __device__ __forceinline__ uint32_t mass_key(float m) {
 // threshold, and writes its part of the list in order.  Keys stay in shared memory between the passes.
 __global__ void __launch_bounds__(EV_THREADS, 1) k_paged_evict_select(const PagedGeom g, const EvictArgs a) {
     extern __shared__ __align__(16) uint32_t ev_smem[];
-    __shared__ int warp_sum[EV_WARPS], warp_gt[EV_WARPS], warp_eq[EV_WARPS], cta_gt, cta_eq, pick[3];
+    __shared__ int warp_sum[EV_WARPS], warp_gt[EV_WARPS], warp_eq[EV_WARPS], pick[2];
+    __shared__ int2 cta_sum;
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     grid_dep_launch();
@@ -128,11 +130,37 @@ __global__ void __launch_bounds__(EV_THREADS, 1) k_paged_evict_select(const Page
     auto key = [&](int i) { return i < EV_KEYS ? keys[i] : read_key(i); };
     for (int i = tid; i < EV_PASSES * EV_BINS; i += EV_THREADS) hist[i] = 0u;
     __syncthreads();
-    for (int i = tid; i < m; i += EV_THREADS) {
-        const uint32_t k = read_key(i);
-        if (i < EV_KEYS) keys[i] = k;
-        if (k) atomicAdd(&hist[k >> (32 - EV_BITS)], 1u);
+    // One count, or one for the whole warp where its keys share a bin (protected positions; equal masses).
+    auto count = [&](uint32_t* h, int bin) {   // whole warps; bin -1: none
+        int same;
+        __match_all_sync(0xffffffffu, bin, &same);
+        if (same) {
+            if (lane == 0 && bin >= 0) atomicAdd(&h[bin], 32u);
+        } else if (bin >= 0) {
+            atomicAdd(&h[bin], 1u);
+        }
+    };
+    for (int i0 = 32 * warp; i0 < m; i0 += EV_HELD * EV_THREADS) {   // EV_HELD positions of a thread in flight
+        int page[EV_HELD], slot[EV_HELD];
+        float x[EV_HELD];
+        bool present[EV_HELD];
+#pragma unroll
+        for (int k = 0; k < EV_HELD; ++k) {
+            const int i = i0 + lane + k * EV_THREADS;
+            present[k] = i < m && g.locate(row, lo + i, page[k], slot[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < EV_HELD; ++k) x[k] = present[k] ? a.mass[g.mass_at(page[k], slot[k], kv)] : 0.0f;
+#pragma unroll
+        for (int k = 0; k < EV_HELD; ++k) {
+            const int i = i0 + lane + k * EV_THREADS, j = lo + i;
+            if (i - lane >= m) break;   // the whole warp
+            const uint32_t y = !present[k] ? 0u : j < a.n_sink || j >= n - a.n_recent ? 0xffffffffu : mass_key(x[k]);
+            if (i < m && i < EV_KEYS) keys[i] = y;
+            count(hist, present[k] ? static_cast<int>(y >> (32 - EV_BITS)) : -1);
+        }
     }
+    __syncthreads();
     // Threshold key and how many positions with exactly that key are kept.  Fewer present positions than
     // n_keep: the scans end in bin 0 with room to spare, the threshold is 0, which absent positions alone have.
     uint32_t prefix = 0u;
@@ -142,9 +170,9 @@ __global__ void __launch_bounds__(EV_THREADS, 1) k_paged_evict_select(const Page
         uint32_t* mine = hist + pass * EV_BINS;
         if (pass > 0) {
             const int above = low + (pass == 1 ? EV_BITS : 32 - 2 * EV_BITS);
-            for (int i = tid; i < m; i += EV_THREADS) {
-                const uint32_t k = key(i);
-                if (k && (k >> above) == (prefix >> above)) atomicAdd(&mine[(k >> low) & (EV_BINS - 1) & ((1u << (above - low)) - 1u)], 1u);
+            for (int i0 = 32 * warp; i0 < m; i0 += EV_THREADS) {
+                const uint32_t k = i0 + lane < m ? key(i0 + lane) : 0u;
+                count(mine, k && (k >> above) == (prefix >> above) ? static_cast<int>(k >> low & ((1u << (above - low)) - 1u)) : -1);
             }
         }
         if (n_cta > 1)
@@ -154,10 +182,16 @@ __global__ void __launch_bounds__(EV_THREADS, 1) k_paged_evict_select(const Page
         // two bins a thread, highest bins first: bins b and b - 1
         const int b = EV_BINS - 1 - 2 * tid;
         int c0 = 0, c1 = 0;
-        for (int r = 0; r < n_cta; ++r) {
-            const uint32_t* h = n_cta > 1 ? cluster.map_shared_rank(mine, r) : mine;
-            c0 += h[b];
-            c1 += h[b - 1];
+        if (n_cta == 1) {
+            c0 = mine[b];
+            c1 = mine[b - 1];
+        } else {
+            uint2 h[EV_MAX_CLUSTER];
+#pragma unroll
+            for (int r = 0; r < EV_MAX_CLUSTER; ++r)
+                h[r] = r < n_cta ? *reinterpret_cast<const uint2*>(cluster.map_shared_rank(mine, r) + b - 1) : make_uint2(0u, 0u);
+#pragma unroll
+            for (int r = 0; r < EV_MAX_CLUSTER; ++r) c0 += h[r].y, c1 += h[r].x;
         }
         int x = c0 + c1;   // inclusive scan over the threads
         for (int o = 1; o < 32; o <<= 1) {
@@ -197,23 +231,22 @@ __global__ void __launch_bounds__(EV_THREADS, 1) k_paged_evict_select(const Page
     }
     if (lane == 0) warp_gt[warp] = gt, warp_eq[warp] = eq;
     __syncthreads();
-    int g0 = 0, e0 = 0;   // before this warp
-    for (int w = 0; w < EV_WARPS; ++w) {
-        if (w == warp && tid != 0) break;
-        if (w < warp) g0 += warp_gt[w], e0 += warp_eq[w];
-        if (tid == 0) cta_gt = (w ? cta_gt : 0) + warp_gt[w], cta_eq = (w ? cta_eq : 0) + warp_eq[w];
-    }
-    int g_all = 0, e_all = 0;
+    // before this warp, and in the whole CTA
+    const int wg = warp_gt[lane], we = warp_eq[lane];
+    int g0 = __reduce_add_sync(0xffffffffu, lane < warp ? wg : 0), e0 = __reduce_add_sync(0xffffffffu, lane < warp ? we : 0);
+    int g_all = __reduce_add_sync(0xffffffffu, wg), e_all = __reduce_add_sync(0xffffffffu, we);
     if (n_cta > 1) {
+        if (tid == 0) cta_sum = make_int2(g_all, e_all);
         cluster.sync();
-        for (int r = 0; r < n_cta; ++r) {
-            const int cg_ = *cluster.map_shared_rank(&cta_gt, r), ce = *cluster.map_shared_rank(&cta_eq, r);
-            if (r < rank) g0 += cg_, e0 += ce;
-            g_all += cg_, e_all += ce;
+        int2 s[EV_MAX_CLUSTER];
+#pragma unroll
+        for (int r = 0; r < EV_MAX_CLUSTER; ++r) s[r] = r < n_cta ? *cluster.map_shared_rank(&cta_sum, r) : make_int2(0, 0);
+        g_all = e_all = 0;
+#pragma unroll
+        for (int r = 0; r < EV_MAX_CLUSTER; ++r) {
+            if (r < rank) g0 += s[r].x, e0 += s[r].y;
+            g_all += s[r].x, e_all += s[r].y;
         }
-    } else {
-        __syncthreads();
-        g_all = cta_gt, e_all = cta_eq;
     }
     for (int i = w0 + lane; i - lane < w1; i += 32) {
         const uint32_t k = i < w1 ? key(i) : 0u;
