@@ -16,7 +16,6 @@ constexpr int LG_THREADS = 512;
 constexpr int LG_HELD = 8;           // logits a thread holds at once: 40 registers, three CTAs per SM
 constexpr int LG_STEP = LG_THREADS * LG_HELD;
 constexpr int LG_SLICE = 4 * LG_STEP;   // tokens whose counters a CTA holds at once (one word each)
-constexpr int LG_LIST = 1024;        // listed tokens that are put aside at once
 constexpr int LG_BATCH = 4;          // list entries of a thread in flight
 constexpr int LG_COUNT_BITS = 20;    // counter word: times in the history; above: last bias entry + 1
 constexpr int LG_MAX_HIST = (1 << LG_COUNT_BITS) - 1, LG_MAX_BIAS = (1 << (32 - LG_COUNT_BITS)) - 2;
@@ -31,18 +30,13 @@ __device__ __forceinline__ void take(Best& a, const Best& b) {
 }
 
 // A cluster of LG_CLUSTER CTAs per row, each with a contiguous share of the vocabulary, LG_SLICE tokens at a
-// time.  The slice's first logits are on their way to registers while the history is counted into
-// shared-memory words (integer atomics: the order does not matter) and each bias entry leaves its index there
-// (the largest, hence the last entry, stays).  Tokens without a word go through at once, only masked.  The
-// others are few and would hold every warp up with their division, so they are put aside and treated together
-// afterwards (beyond LG_LIST of them in a slice, on the spot).  VEC = 4 where all rows are 16-byte aligned,
+// time.  The slice's logits are on their way to L2 while the history is counted into shared-memory words
+// (integer atomics: the order does not matter) and each bias entry leaves its index there (the largest, hence
+// the last entry, stays); then the logits stream past the words.  VEC = 4 where all rows are 16-byte aligned,
 // else 1.
 template <int VEC>
 __global__ void __launch_bounds__(LG_THREADS, 3) k_logits(const mcpm_logits_params p) {
     extern __shared__ __align__(16) uint32_t words[];   // [LG_SLICE]
-    __shared__ float aside_v[LG_LIST];
-    __shared__ uint32_t aside_t[LG_LIST];   // token - s0, bit 31: allowed
-    __shared__ int n_aside;
     __shared__ Best warp_best[LG_THREADS / 32], cta_best[LG_CLUSTER];
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
@@ -63,20 +57,18 @@ __global__ void __launch_bounds__(LG_THREADS, 3) k_logits(const mcpm_logits_para
     float rep = 1.0f, freq = 0.0f, pres = 0.0f;
     if (n_hist) rep = p.penalties[3 * row], freq = p.penalties[3 * row + 1], pres = p.penalties[3 * row + 2];
     Best best{-INFINITY, 0x7fffffff};
-    auto consider = [&](float v, int t) {   // the lowest token of the largest value, whatever the order of calls
-        if (v > best.v || (v == best.v && t < best.t && v > -INFINITY)) best = Best{v, t};
-    };
-    auto listed = [&](float y, uint32_t w, bool ok) {
+    auto listed = [&](float y, uint32_t w) {
         const uint32_t c = w & LG_MAX_HIST, b = w >> LG_COUNT_BITS;
         if (c) {
             y = y > 0.0f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
             y = __fsub_rn(y, __fadd_rn(__fmul_rn(freq, static_cast<float>(c)), pres));
         }
         if (b) y = __fadd_rn(y, p.bias[row * p.bias_stride + b - 1]);
-        return ok ? y : -INFINITY;
+        return y;
     };
     for (int s0 = lo; s0 < hi; s0 += LG_SLICE) {
         const int n = min(LG_SLICE, hi - s0);
+        if (VEC == 4 && tid == 0 && n >= 4) bulk_prefetch_l2(x + s0, (n & ~3) * 4);   // on its way while the lists are counted
         float v[LG_HELD];
         uint32_t bits[LG_HELD / VEC];   // VEC divides 32: a load's tokens share a mask word
         auto load = [&](int c) {
@@ -96,7 +88,6 @@ __global__ void __launch_bounds__(LG_THREADS, 3) k_logits(const mcpm_logits_para
         };
         load(0);
         if (lists) {
-            if (tid == 0) n_aside = 0;
             for (int i = tid; i < (n + 3) / 4; i += LG_THREADS) reinterpret_cast<uint4*>(words)[i] = make_uint4(0u, 0u, 0u, 0u);
             __syncthreads();
             for (int i = tid; i < n_bias; i += LG_THREADS) {
@@ -121,30 +112,30 @@ __global__ void __launch_bounds__(LG_THREADS, 3) k_logits(const mcpm_logits_para
             for (int k = 0; k < LG_HELD / VEC; ++k) {
                 const int i = c + VEC * (k * LG_THREADS + tid);
                 if (i >= n) break;
-                uint32_t w[VEC] = {};
+                float* y = v + VEC * k;
                 if (lists) {
+                    uint32_t w[VEC], any = 0u;
                     if constexpr (VEC == 4)
                         *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(words + i);
                     else
                         w[0] = words[i];
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) any |= w[e];
+                    if (any)
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e)
+                            if (w[e]) y[e] = listed(y[e], w[e]);
                 }
+                float top = -INFINITY;
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
-                    const bool ok = bits[k] >> e & 1u;
-                    float& y = v[VEC * k + e];
-                    if (i + e >= n) continue;
-                    if (w[e]) {
-                        const int at = atomicAdd(&n_aside, 1);
-                        if (at < LG_LIST) {
-                            aside_v[at] = y;
-                            aside_t[at] = static_cast<uint32_t>(i + e) | static_cast<uint32_t>(ok) << 31;
-                            continue;   // its place in out is written again below
-                        }
-                        y = listed(y, w[e], ok);
-                    } else if (!ok) {
-                        y = -INFINITY;
-                    }
-                    if (y > best.v) best = Best{y, s0 + i + e};   // tokens ascend here
+                    if (!(bits[k] >> e & 1u)) y[e] = -INFINITY;
+                    if (i + e < n) top = fmaxf(top, y[e]);   // NaN never
+                }
+                if (top > best.v) {   // seldom; tokens ascend here
+#pragma unroll
+                    for (int e = VEC - 1; e >= 0; --e)
+                        if (i + e < n && y[e] == top) best = Best{top, s0 + i + e};
                 }
                 if (VEC == 4 && i + 3 < n)
                     *reinterpret_cast<float4*>(out + s0 + i) = *reinterpret_cast<const float4*>(v + VEC * k);
@@ -153,16 +144,7 @@ __global__ void __launch_bounds__(LG_THREADS, 3) k_logits(const mcpm_logits_para
                         if (i + e < n) out[s0 + i + e] = v[VEC * k + e];
             }
         }
-        if (lists) {
-            __syncthreads();
-            for (int k = tid; k < min(n_aside, LG_LIST); k += LG_THREADS) {
-                const int i = static_cast<int>(aside_t[k] & 0x7fffffffu);
-                const float y = listed(aside_v[k], words[i], aside_t[k] >> 31);
-                out[s0 + i] = y;
-                consider(y, s0 + i);
-            }
-            __syncthreads();
-        }
+        __syncthreads();   // the words are free
     }
     if (!p.argmax) return;   // the whole grid
     for (int o = 16; o >= 1; o >>= 1)

@@ -88,6 +88,7 @@ constexpr int EV_THREADS = 1024, EV_WARPS = EV_THREADS / 32;
 constexpr int EV_MAX_CLUSTER = 8;
 constexpr int EV_BITS = 11, EV_BINS = 1 << EV_BITS, EV_PASSES = 3;   // digits of 11, 11 and 10 bits, highest first
 constexpr int EV_KEYS = 32768;   // keys a CTA holds in shared memory
+constexpr int EV_RANKED = 512;   // at most EV_THREADS
 constexpr int EV_HELD = 4;       // positions a thread reads at once
 constexpr int EV_SMEM = (EV_PASSES * EV_BINS + EV_KEYS) * 4;
 
@@ -105,7 +106,7 @@ __device__ __forceinline__ uint32_t mass_key(float m) {
 // threshold, and writes its part of the list in order.  Keys stay in shared memory between the passes.
 __global__ void __launch_bounds__(EV_THREADS, 1) k_paged_evict_select(const PagedGeom g, const EvictArgs a) {
     extern __shared__ __align__(16) uint32_t ev_smem[];
-    __shared__ int warp_sum[EV_WARPS], warp_gt[EV_WARPS], warp_eq[EV_WARPS], pick[2];
+    __shared__ int groups[EV_PASSES][EV_BINS / 32], warp_gt[EV_WARPS], warp_eq[EV_WARPS], pick[3];
     __shared__ int2 cta_sum;
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
@@ -175,50 +176,82 @@ __global__ void __launch_bounds__(EV_THREADS, 1) k_paged_evict_select(const Page
                 count(mine, k && (k >> above) == (prefix >> above) ? static_cast<int>(k >> low & ((1u << (above - low)) - 1u)) : -1);
             }
         }
+        __syncthreads();
+        for (int q = warp; q < EV_BINS / 32; q += EV_WARPS) {
+            const int s = __reduce_add_sync(0xffffffffu, mine[32 * q + lane]);
+            if (lane == 0) groups[pass][q] = s;
+        }
         if (n_cta > 1)
             cluster.sync();
         else
             __syncthreads();
-        // two bins a thread, highest bins first: bins b and b - 1
-        const int b = EV_BINS - 1 - 2 * tid;
-        int c0 = 0, c1 = 0;
-        if (n_cta == 1) {
-            c0 = mine[b];
-            c1 = mine[b - 1];
-        } else {
-            uint2 h[EV_MAX_CLUSTER];
+        // The bin in which the count from above reaches `need`, in two steps of 64 groups of 32 bins, so that a
+        // CTA reads 96 words of each of the others' histograms and not all of them.
+        auto from_top = [&](int c, int& before, int& all) {   // lane 0 holds the highest
+            int s = c;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, s, o);
+                if (lane >= o) s += y;
+            }
+            before = s - c;
+            all = __shfl_sync(0xffffffffu, s, 31);
+        };
+        if (warp == 0) {
+            int c[2] = {0, 0}, before[2], all[2];   // groups 63 - lane and 31 - lane
 #pragma unroll
             for (int r = 0; r < EV_MAX_CLUSTER; ++r)
-                h[r] = r < n_cta ? *reinterpret_cast<const uint2*>(cluster.map_shared_rank(mine, r) + b - 1) : make_uint2(0u, 0u);
+                if (r < n_cta) {
+                    const int* h = n_cta > 1 ? cluster.map_shared_rank(groups[pass], r) : groups[pass];
+                    c[0] += h[63 - lane];
+                    c[1] += h[31 - lane];
+                }
+            from_top(c[0], before[0], all[0]);
+            from_top(c[1], before[1], all[1]);
+            before[1] += all[0];
+            const unsigned hit0 = __ballot_sync(0xffffffffu, before[0] < need && before[0] + c[0] >= need);
+            const unsigned hit1 = __ballot_sync(0xffffffffu, before[1] < need && before[1] + c[1] >= need);
+            // fewer positions than needed: bin 0 is taken whole
+            const int group = hit0 ? 63 - (__ffs(hit0) - 1) : hit1 ? 31 - (__ffs(hit1) - 1) : 0;
+            const int above = hit0   ? __shfl_sync(0xffffffffu, before[0], __ffs(hit0) - 1)
+                              : hit1 ? __shfl_sync(0xffffffffu, before[1], __ffs(hit1) - 1)
+                                     : __shfl_sync(0xffffffffu, before[1], 31);
+            int f = 0, fb, fa;
 #pragma unroll
-            for (int r = 0; r < EV_MAX_CLUSTER; ++r) c0 += h[r].y, c1 += h[r].x;
-        }
-        int x = c0 + c1;   // inclusive scan over the threads
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += y;
-        }
-        if (lane == 31) warp_sum[warp] = x;
-        __syncthreads();
-        int w = warp_sum[lane];
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, w, o);
-            if (lane >= o) w += y;
-        }
-        const int all = __shfl_sync(0xffffffffu, w, 31), before_warp = __shfl_sync(0xffffffffu, w, (warp + 31) & 31);
-        const int before = x - c0 - c1 + (warp ? before_warp : 0);   // positions in higher bins
-        if (before < need && before + c0 + c1 >= need) {
-            const bool first = before + c0 >= need;
-            pick[0] = first ? b : b - 1;
-            pick[1] = first ? before : before + c0;
-        } else if (tid == EV_THREADS - 1 && all < need) {   // bin 0 is taken whole
-            pick[0] = 0;
-            pick[1] = all - c1;
+            for (int r = 0; r < EV_MAX_CLUSTER; ++r)
+                if (r < n_cta) f += static_cast<int>((n_cta > 1 ? cluster.map_shared_rank(mine, r) : mine)[32 * group + 31 - lane]);
+            from_top(f, fb, fa);
+            fb += above;
+            const unsigned hit = __ballot_sync(0xffffffffu, fb < need && fb + f >= need);
+            const int at = hit ? __ffs(hit) - 1 : 31;
+            if (lane == at) pick[0] = 32 * group + 31 - lane, pick[1] = fb, pick[2] = hit ? f : EV_THREADS + 1;
         }
         __syncthreads();
         prefix |= static_cast<uint32_t>(pick[0]) << low;
         need -= pick[1];
+        const int in_bin = pick[2];
         __syncthreads();
+        if (n_cta == 1 && in_bin <= EV_RANKED && pass + 1 < EV_PASSES) {
+            // Few keys share the threshold's digits (a few percent of 2048 bins' worth): each is ranked against
+            // the others, in place of the remaining passes.
+            uint32_t* cand = hist + (pass + 1) * EV_BINS;   // zeroed, in_bin <= EV_RANKED entries
+            if (tid == 0) pick[0] = 0;
+            __syncthreads();
+            for (int i = tid; i < m; i += EV_THREADS) {
+                const uint32_t k = key(i);
+                if (k && (k >> low) == (prefix >> low)) cand[atomicAdd(&pick[0], 1)] = k;
+            }
+            __syncthreads();
+            if (tid < in_bin) {
+                const uint32_t k = cand[tid];
+                int above = 0, at = 0;
+                for (int i = 0; i < in_bin; ++i) above += cand[i] > k, at += cand[i] == k;
+                if (above < need && above + at >= need) pick[1] = static_cast<int>(k), pick[2] = need - above;   // equal keys write the same
+            }
+            __syncthreads();
+            prefix = static_cast<uint32_t>(pick[1]);
+            need = pick[2];
+            break;
+        }
     }
     // each warp's contiguous positions: how many are above the threshold, how many at it
     const int per = ((m + EV_WARPS - 1) / EV_WARPS + 31) & ~31;
