@@ -12,13 +12,18 @@ namespace mcpm {
 namespace {
 
 constexpr int LG_CLUSTER = 8;        // CTAs that share a row
-constexpr int LG_THREADS = 512;
-constexpr int LG_HELD = 8;           // logits a thread holds at once: 40 registers, three CTAs per SM
-constexpr int LG_STEP = LG_THREADS * LG_HELD;
-constexpr int LG_SLICE = 4 * LG_STEP;   // tokens whose counters a CTA holds at once (one word each)
-constexpr int LG_BATCH = 4;          // list entries of a thread in flight
-constexpr int LG_COUNT_BITS = 20;    // counter word: times in the history; above: last bias entry + 1
+constexpr int LG_THREADS = 256;
+constexpr int LG_CHUNK_BITS = 10, LG_CHUNK = 1 << LG_CHUNK_BITS;   // tokens that go to one CTA in a row, four a thread
+constexpr int LG_CHUNKS = 16;        // chunks whose words a CTA holds at once
+constexpr int LG_SLICE = LG_CHUNKS * LG_CHUNK;
+constexpr int LG_HELD = 4;           // chunks in registers at once
+constexpr int LG_BATCH = 8;          // history entries of a thread in flight
+constexpr int LG_QUEUE = 2 * LG_BATCH * LG_THREADS;   // history entries of a CTA in one round
+constexpr int LG_LISTED = 1024;      // listed tokens of a slice
+constexpr int LG_COUNT_BITS = 20;    // counter: times in the history; above: last bias entry + 1
 constexpr int LG_MAX_HIST = (1 << LG_COUNT_BITS) - 1, LG_MAX_BIAS = (1 << (32 - LG_COUNT_BITS)) - 2;
+static_assert(LG_CHUNK == 4 * LG_THREADS && LG_SLICE <= 32768 && LG_CHUNKS % LG_HELD == 0, "");
+static_assert(LG_LISTED >= LG_CHUNK, "one chunk's tokens fit the list");
 
 struct Best {
     float v;
@@ -29,14 +34,23 @@ __device__ __forceinline__ void take(Best& a, const Best& b) {
     if (b.v > a.v || (b.v == a.v && b.t < a.t)) a = b;
 }
 
-// A cluster of LG_CLUSTER CTAs per row, each with a contiguous share of the vocabulary, LG_SLICE tokens at a
-// time.  The slice's logits are on their way to L2 while the history is counted into shared-memory words
-// (integer atomics: the order does not matter) and each bias entry leaves its index there (the largest, hence
-// the last entry, stays); then the logits stream past the words.  VEC = 4 where all rows are 16-byte aligned,
-// else 1.
-template <int VEC>
-__global__ void __launch_bounds__(LG_THREADS, 3) k_logits(const mcpm_logits_params p) {
-    extern __shared__ __align__(16) uint32_t words[];   // [LG_SLICE]
+// A cluster of LG_CLUSTER CTAs per row.  Chunks of the vocabulary go to them in turn: frequent tokens have low
+// ids, and with contiguous shares the first CTA had half of a long history (64 rows with 4096 tokens each: 35 us).
+// Per LG_SLICE tokens of a CTA: every thread passes over a share of the history and queues the entries that are
+// this CTA's (an eighth: worked on in place they would keep every warp busy for a few lanes).  The queued tokens
+// claim their 16-bit words, the first of each takes a place on a list, and then every entry counts at its
+// token's place and every bias entry leaves its index there (integer atomics: the order does not matter; the
+// largest index is the last entry).  The streaming pass puts the logits of listed tokens aside, and they are
+// computed side by side after it.  A slice with more listed tokens than the list holds is cut in half until
+// they fit.  VEC = 4 where all rows are 16-byte aligned, else 1.
+template <int VEC, bool LISTS, bool MASK>
+__global__ void __launch_bounds__(LG_THREADS, 4) k_logits(const mcpm_logits_params p) {
+    extern __shared__ __align__(16) uint16_t words[];    // [LG_SLICE] place on the list plus 1; zero: not listed
+    __shared__ uint32_t counts[LISTS ? LG_LISTED : 1];   // the counters of the listed tokens
+    __shared__ float aside[LISTS ? LG_LISTED : 1];       // their logits
+    __shared__ uint16_t list[LISTS ? LG_LISTED : 1];     // their places in the slice
+    __shared__ uint16_t queue[LISTS ? LG_QUEUE : 1];
+    __shared__ int n_list, n_queue;
     __shared__ Best warp_best[LG_THREADS / 32], cta_best[LG_CLUSTER];
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
@@ -44,107 +58,203 @@ __global__ void __launch_bounds__(LG_THREADS, 3) k_logits(const mcpm_logits_para
     grid_dep_launch();
     grid_dep_wait();
     const int tid = threadIdx.x, rank = cluster.block_rank(), row = blockIdx.x / LG_CLUSTER;
-    const int share = ((p.n_vocab + LG_CLUSTER - 1) / LG_CLUSTER + 31) & ~31;   // whole mask words
-    const int lo = min(p.n_vocab, rank * share), hi = min(p.n_vocab, lo + share);
+    const int V = p.n_vocab;
     const float* x = p.logits + row * p.logits_stride;
     float* out = p.out + row * p.out_stride;
-    const int* hist = p.hist ? p.hist + row * p.hist_stride : nullptr;
-    const int n_hist = hist ? (p.hist_len ? min(max(p.hist_len[row], 0), p.hist_max) : p.hist_max) : 0;
-    const int* bias_token = p.bias_token ? p.bias_token + row * p.bias_stride : nullptr;
-    const int n_bias = bias_token ? (p.bias_len ? min(max(p.bias_len[row], 0), p.bias_max) : p.bias_max) : 0;
-    const uint32_t* allow = p.allow ? p.allow + row * p.allow_stride : nullptr;
-    const bool lists = n_hist || n_bias;
-    float rep = 1.0f, freq = 0.0f, pres = 0.0f;
-    if (n_hist) rep = p.penalties[3 * row], freq = p.penalties[3 * row + 1], pres = p.penalties[3 * row + 2];
+    const uint32_t* allow = MASK ? p.allow + row * p.allow_stride : nullptr;
+    // chunk k of this CTA begins at token base_of(k); a thread's tokens of it are place(0 .. 3) further
+    auto base_of = [&](int k) { return (k * LG_CLUSTER + rank) << LG_CHUNK_BITS; };
+    auto place = [&](int e) { return VEC == 4 ? 4 * tid + e : e * LG_THREADS + tid; };
+    const int mine = (((V + LG_CHUNK - 1) >> LG_CHUNK_BITS) - rank + LG_CLUSTER - 1) / LG_CLUSTER;   // chunks of this CTA
     Best best{-INFINITY, 0x7fffffff};
+    float v[LG_HELD][4];
+    uint32_t bits[LG_HELD][VEC == 4 ? 1 : 4];   // the mask words of the thread's tokens
+    auto load = [&](int k0) {
+#pragma unroll
+        for (int k = 0; k < LG_HELD; ++k) {
+            const int base = base_of(k0 + k);
+            if (base + LG_CHUNK <= V) {
+                if constexpr (VEC == 4) {
+                    *reinterpret_cast<float4*>(v[k]) = *reinterpret_cast<const float4*>(x + base + 4 * tid);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[k][e] = x[base + place(e)];
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[k][e] = base + place(e) < V ? x[base + place(e)] : -INFINITY;
+            }
+        }
+        if constexpr (MASK) {
+#pragma unroll
+            for (int k = 0; k < LG_HELD; ++k)
+#pragma unroll
+                for (int e = 0; e < (VEC == 4 ? 1 : 4); ++e) {
+                    const int t = base_of(k0 + k) + place(e);
+                    bits[k][e] = t < V ? allow[t >> 5] : 0u;
+                }
+        }
+    };
+    const int* hist = LISTS && p.hist ? p.hist + row * p.hist_stride : nullptr;
+    const int* bias_token = LISTS && p.bias_token ? p.bias_token + row * p.bias_stride : nullptr;
+    int n_hist = hist ? p.hist_max : 0, n_bias = bias_token ? p.bias_max : 0;
+    float rep = 1.0f, freq = 0.0f, pres = 0.0f;
+    int first_bias = -1;
+    if constexpr (LISTS) {
+        if (tid < n_bias) first_bias = bias_token[tid];
+        if (hist && p.hist_len) n_hist = min(max(p.hist_len[row], 0), p.hist_max);
+        if (bias_token && p.bias_len) n_bias = min(max(p.bias_len[row], 0), p.bias_max);
+        if (hist) rep = p.penalties[3 * row], freq = p.penalties[3 * row + 1], pres = p.penalties[3 * row + 2];
+    }
     auto listed = [&](float y, uint32_t w) {
         const uint32_t c = w & LG_MAX_HIST, b = w >> LG_COUNT_BITS;
         if (c) {
             y = y > 0.0f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
             y = __fsub_rn(y, __fadd_rn(__fmul_rn(freq, static_cast<float>(c)), pres));
         }
-        if (b) y = __fadd_rn(y, p.bias[row * p.bias_stride + b - 1]);
-        return y;
+        return b ? __fadd_rn(y, p.bias[row * p.bias_stride + b - 1]) : y;
     };
-    for (int s0 = lo; s0 < hi; s0 += LG_SLICE) {
-        const int n = min(LG_SLICE, hi - s0);
-        if (VEC == 4 && tid == 0 && n >= 4) bulk_prefetch_l2(x + s0, (n & ~3) * 4);   // on its way while the lists are counted
-        float v[LG_HELD];
-        uint32_t bits[LG_HELD / VEC];   // VEC divides 32: a load's tokens share a mask word
-        auto load = [&](int c) {
+    for (int c0 = 0, c1; c0 < mine; c0 = c1) {
+        c1 = min(mine, c0 + LG_CHUNKS);
+        if constexpr (LISTS) {
+            // the first logits come to registers meanwhile, the others to L2
+            load(c0);
+            if (VEC == 4 && tid >= LG_HELD && tid < c1 - c0 && base_of(c0 + tid) + LG_CHUNK <= V)
+                bulk_prefetch_l2(x + base_of(c0 + tid), LG_CHUNK * 4);
+            const int lane = tid & 31;
+            // the word of a token, if it is in this slice
+            auto word_of = [&](int token) -> unsigned {
+                const unsigned chunk = static_cast<unsigned>(token) >> LG_CHUNK_BITS, k = chunk / LG_CLUSTER - c0;
+                const bool here = chunk % LG_CLUSTER == rank && k < static_cast<unsigned>(c1 - c0) && token < V;   // a negative token's chunk lies beyond
+                return here ? k << LG_CHUNK_BITS | (token & (LG_CHUNK - 1)) : ~0u;
+            };
+            auto claim = [&](unsigned w) {
+                if (words[w] || atomicCAS(&words[w], static_cast<unsigned short>(0), static_cast<unsigned short>(0xffff))) return;
+                const int at = atomicAdd(&n_list, 1);
+                if (at < LG_LISTED) {
+                    list[at] = static_cast<uint16_t>(w);
+                    counts[at] = 0u;
+                    words[w] = static_cast<uint16_t>(at + 1);   // read after a barrier
+                }
+            };
+            for (bool again = true; again;) {
+                if (tid == 0) n_list = n_queue = 0;
+                for (int i = tid; i < (c1 - c0) * LG_CHUNK / 8; i += LG_THREADS) reinterpret_cast<uint4*>(words)[i] = make_uint4(0u, 0u, 0u, 0u);
+                __syncthreads();
+                auto each_bias = [&](auto f) {
+                    for (int i = tid; i < n_bias; i += LG_THREADS) {
+                        const unsigned w = word_of(i < LG_THREADS ? first_bias : bias_token[i]);
+                        if (w != ~0u) f(i, w);
+                    }
+                };
+                each_bias([&](int, unsigned w) { claim(w); });
+                again = false;
+                for (int r0 = 0; r0 == 0 || (r0 < n_hist && !again); r0 += LG_QUEUE) {   // rounds
+                    for (int b0 = r0; b0 < min(n_hist, r0 + LG_QUEUE); b0 += LG_BATCH * LG_THREADS) {
+                        unsigned w[LG_BATCH];
+                        int before[LG_BATCH], sum = 0;
 #pragma unroll
-            for (int k = 0; k < LG_HELD / VEC; ++k) {
-                const int i = c + VEC * (k * LG_THREADS + tid);
-                if (VEC == 4 && i + 3 < n)
-                    *reinterpret_cast<float4*>(v + VEC * k) = *reinterpret_cast<const float4*>(x + s0 + i);
-                else
-                    for (int e = 0; e < VEC; ++e) v[VEC * k + e] = i + e < n ? x[s0 + i + e] : 0.0f;
-            }
+                        for (int k = 0; k < LG_BATCH; ++k) {
+                            const int i = b0 + k * LG_THREADS + tid;
+                            w[k] = static_cast<unsigned>(i < n_hist ? hist[i] : -1);
+                        }
 #pragma unroll
-            for (int k = 0; k < LG_HELD / VEC; ++k) {
-                const int i = c + VEC * (k * LG_THREADS + tid);
-                bits[k] = allow && i < n ? allow[(s0 + i) >> 5] >> ((s0 + i) & 31) : 0xffffffffu;
-            }
-        };
-        load(0);
-        if (lists) {
-            for (int i = tid; i < (n + 3) / 4; i += LG_THREADS) reinterpret_cast<uint4*>(words)[i] = make_uint4(0u, 0u, 0u, 0u);
-            __syncthreads();
-            for (int i = tid; i < n_bias; i += LG_THREADS) {
-                const unsigned t = static_cast<unsigned>(bias_token[i]) - static_cast<unsigned>(s0);
-                if (t < static_cast<unsigned>(n)) atomicMax(&words[t], static_cast<uint32_t>(i + 1) << LG_COUNT_BITS);
-            }
-            if (n_bias) __syncthreads();   // the maximum is taken of whole words: no counts in them yet
-            for (int i0 = tid; i0 < n_hist; i0 += LG_BATCH * LG_THREADS) {
-                unsigned t[LG_BATCH];
+                        for (int k = 0; k < LG_BATCH; ++k) {
+                            w[k] = word_of(static_cast<int>(w[k]));
+                            const unsigned m = __ballot_sync(0xffffffffu, w[k] != ~0u);
+                            before[k] = sum + __popc(m & ((1u << lane) - 1u));
+                            sum += __popc(m);
+                        }
+                        int at = 0;
+                        if (lane == 0 && sum) at = atomicAdd(&n_queue, sum);
+                        at = __shfl_sync(0xffffffffu, at, 0);
 #pragma unroll
-                for (int k = 0; k < LG_BATCH; ++k)
-                    t[k] = i0 + k * LG_THREADS < n_hist ? static_cast<unsigned>(hist[i0 + k * LG_THREADS]) - static_cast<unsigned>(s0) : ~0u;
-#pragma unroll
-                for (int k = 0; k < LG_BATCH; ++k)
-                    if (t[k] < static_cast<unsigned>(n)) atomicAdd(&words[t[k]], 1u);
+                        for (int k = 0; k < LG_BATCH; ++k)
+                            if (w[k] != ~0u) queue[at + before[k]] = static_cast<uint16_t>(w[k]);
+                    }
+                    __syncthreads();
+                    const int n = n_queue;
+                    for (int i = tid; i < n; i += LG_THREADS) claim(queue[i]);
+                    __syncthreads();
+                    again = n_list > LG_LISTED;
+                    if (!again) {
+                        for (int i = tid; i < n; i += LG_THREADS) atomicAdd(&counts[words[queue[i]] - 1], 1u);
+                        if (r0 == 0)
+                            each_bias([&](int i, unsigned w) {   // the largest index, beside a count that others add to
+                                uint32_t* c = &counts[words[w] - 1];
+                                const uint32_t mark = static_cast<uint32_t>(i + 1);
+                                for (uint32_t old = *c; (old >> LG_COUNT_BITS) < mark;) {   // each failure is another's success
+                                    const uint32_t seen = atomicCAS(c, old, mark << LG_COUNT_BITS | (old & LG_MAX_HIST));
+                                    if (seen == old) break;
+                                    old = seen;
+                                }
+                            });
+                    }
+                    if (tid == 0) n_queue = 0;
+                    __syncthreads();
+                }
+                if (again) c1 = c0 + (c1 - c0 + 1) / 2;   // ends: a chunk's tokens fit the list
             }
-            __syncthreads();
         }
-        for (int c = 0; c < n; c += LG_STEP) {
-            if (c) load(c);
+        if (!LISTS) load(c0);
+        for (int k0 = c0; k0 < c1; k0 += LG_HELD) {
+            if (k0 > c0) load(k0);
 #pragma unroll
-            for (int k = 0; k < LG_HELD / VEC; ++k) {
-                const int i = c + VEC * (k * LG_THREADS + tid);
-                if (i >= n) break;
-                float* y = v + VEC * k;
-                if (lists) {
-                    uint32_t w[VEC], any = 0u;
-                    if constexpr (VEC == 4)
-                        *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(words + i);
-                    else
-                        w[0] = words[i];
+            for (int k = 0; k < LG_HELD; ++k) {
+                if (k0 + k >= c1) break;
+                float* y = v[k];
+                const int base = base_of(k0 + k);
+                if constexpr (MASK) {
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e) any |= w[e];
-                    if (any)
-#pragma unroll
-                        for (int e = 0; e < VEC; ++e)
-                            if (w[e]) y[e] = listed(y[e], w[e]);
+                    for (int e = 0; e < 4; ++e)
+                        if (!(bits[k][VEC == 4 ? 0 : e] >> (place(e) & 31) & 1u)) y[e] = -INFINITY;   // base is a multiple of 32
                 }
-                float top = -INFINITY;
+                if constexpr (LISTS) {
+                    const uint16_t* w = words + ((k0 + k - c0) << LG_CHUNK_BITS);
+                    uint16_t z[4];
+                    if constexpr (VEC == 4) {
+                        *reinterpret_cast<uint2*>(z) = reinterpret_cast<const uint2*>(w)[tid];
+                    } else {
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    if (!(bits[k] >> e & 1u)) y[e] = -INFINITY;
-                    if (i + e < n) top = fmaxf(top, y[e]);   // NaN never
-                }
-                if (top > best.v) {   // seldom; tokens ascend here
+                        for (int e = 0; e < 4; ++e) z[e] = w[place(e)];
+                    }
 #pragma unroll
-                    for (int e = VEC - 1; e >= 0; --e)
-                        if (i + e < n && y[e] == top) best = Best{top, s0 + i + e};
+                    for (int e = 0; e < 4; ++e) {
+                        if (z[e]) aside[z[e] - 1] = y[e];
+                        y[e] = z[e] ? -INFINITY : y[e];   // not a candidate yet; its place in out is written again below
+                    }
                 }
-                if (VEC == 4 && i + 3 < n)
-                    *reinterpret_cast<float4*>(out + s0 + i) = *reinterpret_cast<const float4*>(v + VEC * k);
-                else
-                    for (int e = 0; e < VEC; ++e)
-                        if (i + e < n) out[s0 + i + e] = v[VEC * k + e];
+                const float top = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]));   // NaN never
+                if (top > best.v) {   // seldom; a thread's tokens ascend
+#pragma unroll
+                    for (int e = 3; e >= 0; --e)
+                        if (y[e] == top) best = Best{top, base + place(e)};
+                }
+                if (base + LG_CHUNK <= V) {
+                    if constexpr (VEC == 4) {
+                        *reinterpret_cast<float4*>(out + base + 4 * tid) = *reinterpret_cast<const float4*>(y);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) out[base + place(e)] = y[e];
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (base + place(e) < V) out[base + place(e)] = y[e];
+                }
             }
         }
-        __syncthreads();   // the words are free
+        if constexpr (LISTS) {
+            __syncthreads();
+            for (int k = tid; k < n_list; k += LG_THREADS) {
+                const int i = list[k], t = base_of(c0 + (i >> LG_CHUNK_BITS)) + (i & (LG_CHUNK - 1));
+                float y = listed(aside[k], counts[k]);   // the mask's -inf stays -inf, unless it meets an infinite penalty or bias
+                if (MASK && y != y && !(allow[t >> 5] >> (t & 31) & 1u)) y = -INFINITY;
+                out[t] = y;
+                if (y > best.v || (y == best.v && t < best.t && y > -INFINITY)) best = Best{y, t};
+            }
+            __syncthreads();   // the words are free
+        }
     }
     if (!p.argmax) return;   // the whole grid
     for (int o = 16; o >= 1; o >>= 1)
@@ -155,8 +265,10 @@ __global__ void __launch_bounds__(LG_THREADS, 3) k_logits(const mcpm_logits_para
         for (int w = 1; w < LG_THREADS / 32; ++w) take(best, warp_best[w]);
     cluster.barrier_wait();   // every CTA of the row has started
     if (tid == 0) *cluster.map_shared_rank(&cta_best[rank], 0) = best;
-    cluster.sync();
-    if (rank == 0 && tid == 0) {
+    cluster.barrier_arrive();
+    if (rank) return;         // only the first CTA waits for the others
+    cluster.barrier_wait();
+    if (tid == 0) {
         for (int c = 1; c < LG_CLUSTER; ++c) take(best, cta_best[c]);
         p.argmax[row] = best.t == 0x7fffffff ? -1 : best.t;
     }
@@ -184,10 +296,14 @@ extern "C" mcpm_status mcpm_logits_process(const mcpm_logits_params* params, voi
     if (p.bias_token && (!p.bias || p.bias_max < 0 || p.bias_max > LG_MAX_BIAS || p.bias_stride < p.bias_max)) return MCPM_BAD_ARG;
     if (p.allow && p.allow_stride < mask_words) return MCPM_BAD_ARG;
     auto aligned = [](const float* q, int64_t stride) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0 && stride % 4 == 0; };
-    void (*kernel)(mcpm_logits_params) =
-        aligned(p.logits, p.logits_stride) && aligned(p.out, p.out_stride) ? k_logits<4> : k_logits<1>;
-    const size_t smem = p.hist || p.bias_token ? LG_SLICE * 4 : 0;
-    cudaError_t e = smem ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LG_SLICE * 4) : cudaSuccess;
+    const bool lists = p.hist || p.bias_token, mask = p.allow != nullptr;
+    void (*kernel)(mcpm_logits_params) = aligned(p.logits, p.logits_stride) && aligned(p.out, p.out_stride)
+                                             ? lists ? mask ? k_logits<4, true, true> : k_logits<4, true, false>
+                                               : mask ? k_logits<4, false, true> : k_logits<4, false, false>
+                                             : lists ? mask ? k_logits<1, true, true> : k_logits<1, true, false>
+                                               : mask ? k_logits<1, false, true> : k_logits<1, false, false>;
+    const size_t smem = lists ? LG_SLICE * sizeof(uint16_t) : 0;
+    cudaError_t e = smem ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) : cudaSuccess;
     if (e == cudaSuccess) {
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(static_cast<unsigned>(p.n_seq) * LG_CLUSTER);
