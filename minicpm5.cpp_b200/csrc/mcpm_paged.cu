@@ -89,7 +89,7 @@ constexpr int EV_MAX_CLUSTER = 8;
 constexpr int EV_BITS = 11, EV_BINS = 1 << EV_BITS, EV_PASSES = 3;   // digits of 11, 11 and 10 bits, highest first
 constexpr int EV_KEYS = 32768;   // keys a CTA holds in shared memory
 constexpr int EV_RANKED = 512;   // at most EV_THREADS
-constexpr int EV_HELD = 4;       // positions a thread reads at once
+constexpr int EV_HELD = 8;       // positions a thread reads at once
 constexpr int EV_SMEM = (EV_PASSES * EV_BINS + EV_KEYS) * 4;
 
 // Order-preserving unsigned key of a position: a larger key is kept first.  Absent positions 0, NaN 1
@@ -110,8 +110,8 @@ __global__ void __launch_bounds__(EV_THREADS, 1) k_paged_evict_select(const Page
     __shared__ int2 cta_sum;
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
-    grid_dep_launch();
     grid_dep_wait();
+    grid_dep_launch();   // after the wait: see k_paged_evict_copy
     uint32_t* hist = ev_smem;   // [EV_PASSES][EV_BINS]
     uint32_t* keys = ev_smem + EV_PASSES * EV_BINS;
     const int n_cta = cluster.num_blocks(), rank = cluster.block_rank();
@@ -133,33 +133,37 @@ __global__ void __launch_bounds__(EV_THREADS, 1) k_paged_evict_select(const Page
     __syncthreads();
     // One count, or one for the whole warp where its keys share a bin (protected positions; equal masses).
     auto count = [&](uint32_t* h, int bin) {   // whole warps; bin -1: none
-        int same;
-        __match_all_sync(0xffffffffu, bin, &same);
+        const unsigned some = __ballot_sync(0xffffffffu, bin >= 0);
+        int same = 0;
+        if (some == 0xffffffffu) __match_all_sync(0xffffffffu, bin, &same);
         if (same) {
-            if (lane == 0 && bin >= 0) atomicAdd(&h[bin], 32u);
+            if (lane == 0) atomicAdd(&h[bin], 32u);
         } else if (bin >= 0) {
             atomicAdd(&h[bin], 1u);
         }
     };
     for (int i0 = 32 * warp; i0 < m; i0 += EV_HELD * EV_THREADS) {   // EV_HELD positions of a thread in flight
+        const int batch = min(EV_HELD, (m - i0 + EV_THREADS - 1) / EV_THREADS);   // of the warp
         int page[EV_HELD], slot[EV_HELD];
         float x[EV_HELD];
         bool present[EV_HELD];
 #pragma unroll
-        for (int k = 0; k < EV_HELD; ++k) {
-            const int i = i0 + lane + k * EV_THREADS;
-            present[k] = i < m && g.locate(row, lo + i, page[k], slot[k]);
-        }
+        for (int k = 0; k < EV_HELD; ++k)
+            if (k < batch) {
+                const int i = i0 + lane + k * EV_THREADS;
+                present[k] = i < m && g.locate(row, lo + i, page[k], slot[k]);
+            }
 #pragma unroll
-        for (int k = 0; k < EV_HELD; ++k) x[k] = present[k] ? a.mass[g.mass_at(page[k], slot[k], kv)] : 0.0f;
+        for (int k = 0; k < EV_HELD; ++k)
+            if (k < batch) x[k] = present[k] ? a.mass[g.mass_at(page[k], slot[k], kv)] : 0.0f;
 #pragma unroll
-        for (int k = 0; k < EV_HELD; ++k) {
-            const int i = i0 + lane + k * EV_THREADS, j = lo + i;
-            if (i - lane >= m) break;   // the whole warp
-            const uint32_t y = !present[k] ? 0u : j < a.n_sink || j >= n - a.n_recent ? 0xffffffffu : mass_key(x[k]);
-            if (i < m && i < EV_KEYS) keys[i] = y;
-            count(hist, present[k] ? static_cast<int>(y >> (32 - EV_BITS)) : -1);
-        }
+        for (int k = 0; k < EV_HELD; ++k)
+            if (k < batch) {
+                const int i = i0 + lane + k * EV_THREADS, j = lo + i;
+                const uint32_t y = !present[k] ? 0u : j < a.n_sink || j >= n - a.n_recent ? 0xffffffffu : mass_key(x[k]);
+                if (i < m && i < EV_KEYS) keys[i] = y;
+                count(hist, present[k] ? static_cast<int>(y >> (32 - EV_BITS)) : -1);
+            }
     }
     __syncthreads();
     // Threshold key and how many positions with exactly that key are kept.  Fewer present positions than
@@ -301,16 +305,17 @@ constexpr int EV_ROWS = 8, EV_COPY_WARPS = 4;
 template <typename T, int D>
 __global__ void __launch_bounds__(32 * EV_COPY_WARPS) k_paged_evict_copy(const PagedGeom g, const EvictArgs a) {
     constexpr int CH = D * static_cast<int>(sizeof(T)) / 16, ITEMS = EV_ROWS * 2 * CH / 32;   // chunks of a row; 16-byte copies a lane
-    grid_dep_launch();
-    grid_dep_wait();
     const int i0 = (blockIdx.x * EV_COPY_WARPS + (threadIdx.x >> 5)) * EV_ROWS, kv = blockIdx.y, seq = blockIdx.z;
     const int lane = threadIdx.x & 31, i = i0 + lane;
+    int sp, ss, dp = 0, ds = 0;
+    // the table is final: the selection before this kernel lets it start only after its own wait
+    const bool dst = lane < EV_ROWS && i < a.n_keep && g.locate(a.dst + static_cast<size_t>(seq) * g.max_pages, i, dp, ds);
+    grid_dep_wait();
+    grid_dep_launch();
     if (i0 >= a.n_keep) return;
     long long from = -1, to = -1;
     if (lane < EV_ROWS && i < a.n_keep) {
         const int j = a.kept[(static_cast<size_t>(seq) * g.n_head_kv + kv) * a.n_keep + i];
-        int sp, ss, dp, ds;
-        const bool dst = g.locate(a.dst + static_cast<size_t>(seq) * g.max_pages, i, dp, ds);
         if (j >= 0 && dst && g.locate(a.table + static_cast<size_t>(seq) * g.max_pages, j, sp, ss)) {
             from = g.row(sp, ss, kv);
             to = g.row(dp, ds, kv);

@@ -350,10 +350,10 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
     const int rec = 2 * PAGED_MAX_GROUP + group * D;   // floats of a record
     auto arrive = [&](int level, int slot, int members) {   // thread 0, after the CTA's stores and a barrier
         unsigned* c = a.cnt + level * 2 * PAGED_MAX_CTAS + slot;
-        __threadfence();
-        const bool last = atomicAdd(c, 1u) == static_cast<unsigned>(members - 1);
+        unsigned before;   // release of the CTA's record, acquire of the others'
+        asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(c) : "memory");
+        const bool last = before == static_cast<unsigned>(members - 1);
         if (last) *c = 0u;
-        __threadfence();
         return last;
     };
     struct Shared {   // a pair of CTAs first .. first + np - 1, this one's record being the k-th
@@ -375,12 +375,13 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
                 const bool mine = i == i0 + lane;
                 float top = -INFINITY, sum = 0.0f;
                 float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                constexpr int TOGETHER = L::CTAS == 1 ? FAN : 8;   // records whose loads are in flight
 #pragma unroll 1
-                for (int j0 = 0; j0 < members; j0 += 8) {   // eight records' loads in flight
-                    float mr[8], lr[8];
-                    float4 r[8];
+                for (int j0 = 0; j0 < members; j0 += TOGETHER) {
+                    float mr[TOGETHER], lr[TOGETHER];
+                    float4 r[TOGETHER];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
+                    for (int j = 0; j < TOGETHER; ++j) {
                         mr[j] = -INFINITY, lr[j] = 0.0f, r[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                         if (j0 + j < members) {
                             const float* p = a.part + static_cast<size_t>(slot_of(s, at + ((j0 + j) << FAN_BITS * level))) * rec;
@@ -391,13 +392,13 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
                     }
                     float to_top = top;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) to_top = fmaxf(to_top, mr[j]);
+                    for (int j = 0; j < TOGETHER; ++j) to_top = fmaxf(to_top, mr[j]);
                     const float keep = top == -INFINITY ? 0.0f : fast_exp2(top - to_top);
                     sum *= keep;
                     x = make_float4(x.x * keep, x.y * keep, x.z * keep, x.w * keep);
                     top = to_top;
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
+                    for (int j = 0; j < TOGETHER; ++j) {
                         const float e = mr[j] == -INFINITY ? 0.0f : fast_exp2(mr[j] - top);
                         sum = fmaf(lr[j], e, sum);
                         x = make_float4(fmaf(r[j].x, e, x.x), fmaf(r[j].y, e, x.y), fmaf(r[j].z, e, x.z), fmaf(r[j].w, e, x.w));
