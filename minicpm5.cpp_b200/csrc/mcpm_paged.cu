@@ -85,7 +85,7 @@ struct EvictArgs {
 };
 
 constexpr int EV_THREADS = 1024, EV_WARPS = EV_THREADS / 32;
-constexpr int EV_MAX_CLUSTER = 8;
+constexpr int EV_MAX_CLUSTER = 16;   // beyond the portable 8: one GPC's SMs
 constexpr int EV_BITS = 11, EV_BINS = 1 << EV_BITS, EV_PASSES = 3;   // digits of 11, 11 and 10 bits, highest first
 constexpr int EV_KEYS = 32768;   // keys a CTA holds in shared memory
 constexpr int EV_RANKED = 512;   // at most EV_THREADS
@@ -106,7 +106,7 @@ __device__ __forceinline__ uint32_t mass_key(float m) {
 // threshold, and writes its part of the list in order.  Keys stay in shared memory between the passes.
 __global__ void __launch_bounds__(EV_THREADS, 1) k_paged_evict_select(const PagedGeom g, const EvictArgs a) {
     extern __shared__ __align__(16) uint32_t ev_smem[];
-    __shared__ int groups[EV_PASSES][EV_BINS / 32], warp_gt[EV_WARPS], warp_eq[EV_WARPS], pick[3];
+    __shared__ int groups[EV_PASSES][EV_BINS / 32], warp_gt[EV_WARPS], warp_eq[EV_WARPS], pick[3], n_cand;
     __shared__ int2 cta_sum;
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
@@ -234,27 +234,39 @@ __global__ void __launch_bounds__(EV_THREADS, 1) k_paged_evict_select(const Page
         need -= pick[1];
         const int in_bin = pick[2];
         __syncthreads();
-        if (n_cta == 1 && in_bin <= EV_RANKED && pass + 1 < EV_PASSES) {
-            // Few keys share the threshold's digits (a few percent of 2048 bins' worth): each is ranked against
-            // the others, in place of the remaining passes.
-            uint32_t* cand = hist + (pass + 1) * EV_BINS;   // zeroed, in_bin <= EV_RANKED entries
-            if (tid == 0) pick[0] = 0;
+        if (in_bin <= EV_RANKED && pass + 1 < EV_PASSES) {
+            // Few keys share the threshold's digits (2^-11 of the keys' spread, then 2^-22): the CTAs list theirs
+            // and each key is ranked against the others, in place of the remaining passes.
+            uint32_t* cand = hist + (pass + 1) * EV_BINS;   // zeroed; this CTA's, then behind EV_RANKED all of them
+            if (tid == 0) n_cand = 0;
             __syncthreads();
             for (int i = tid; i < m; i += EV_THREADS) {
                 const uint32_t k = key(i);
-                if (k && (k >> low) == (prefix >> low)) cand[atomicAdd(&pick[0], 1)] = k;
+                if (k && (k >> low) == (prefix >> low)) cand[atomicAdd(&n_cand, 1)] = k;
+            }
+            const uint32_t* all = cand;
+            if (n_cta > 1) {
+                cluster.sync();
+                if (warp < n_cta && lane == 0) warp_gt[warp] = *cluster.map_shared_rank(&n_cand, warp);
+                __syncthreads();
+                if (warp < n_cta) {   // a warp per CTA's list; in_bin entries in all
+                    const int c = warp_gt[warp], at = __reduce_add_sync(0xffffffffu, lane < warp ? warp_gt[lane] : 0);
+                    const uint32_t* theirs = cluster.map_shared_rank(cand, warp);
+                    for (int i = lane; i < c; i += 32) cand[EV_RANKED + at + i] = theirs[i];
+                }
+                all = cand + EV_RANKED;
             }
             __syncthreads();
             if (tid < in_bin) {
-                const uint32_t k = cand[tid];
+                const uint32_t k = all[tid];
                 int above = 0, at = 0;
-                for (int i = 0; i < in_bin; ++i) above += cand[i] > k, at += cand[i] == k;
+                for (int i = 0; i < in_bin; ++i) above += all[i] > k, at += all[i] == k;
                 if (above < need && above + at >= need) pick[1] = static_cast<int>(k), pick[2] = need - above;   // equal keys write the same
             }
             __syncthreads();
             prefix = static_cast<uint32_t>(pick[1]);
             need = pick[2];
-            break;
+            break;   // other CTAs may still read this one's list: the next cluster barrier comes before any reuse
         }
     }
     // each warp's contiguous positions: how many are above the threshold, how many at it
@@ -275,15 +287,15 @@ __global__ void __launch_bounds__(EV_THREADS, 1) k_paged_evict_select(const Page
     if (n_cta > 1) {
         if (tid == 0) cta_sum = make_int2(g_all, e_all);
         cluster.sync();
-        int2 s[EV_MAX_CLUSTER];
-#pragma unroll
-        for (int r = 0; r < EV_MAX_CLUSTER; ++r) s[r] = r < n_cta ? *cluster.map_shared_rank(&cta_sum, r) : make_int2(0, 0);
-        g_all = e_all = 0;
-#pragma unroll
-        for (int r = 0; r < EV_MAX_CLUSTER; ++r) {
-            if (r < rank) g0 += s[r].x, e0 += s[r].y;
-            g_all += s[r].x, e_all += s[r].y;
+        if (warp == 0) {
+            const int2 s = lane < n_cta ? *cluster.map_shared_rank(&cta_sum, lane) : make_int2(0, 0);
+            const int gb = __reduce_add_sync(0xffffffffu, lane < rank ? s.x : 0), eb = __reduce_add_sync(0xffffffffu, lane < rank ? s.y : 0);
+            const int ga = __reduce_add_sync(0xffffffffu, s.x), ea = __reduce_add_sync(0xffffffffu, s.y);
+            if (lane == 0) pick[0] = gb, pick[1] = eb, pick[2] = ga, n_cand = ea;
         }
+        __syncthreads();
+        g0 += pick[0], e0 += pick[1];
+        g_all = pick[2], e_all = n_cand;
     }
     for (int i = w0 + lane; i - lane < w1; i += 32) {
         const uint32_t k = i < w1 ? key(i) : 0u;
@@ -357,6 +369,7 @@ cudaError_t launch_evict_select(const PagedGeom& g, const EvictArgs& a, int n_se
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
     if (!prepared[dev]) {
         e = cudaFuncSetAttribute(k_paged_evict_select, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_SMEM);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(k_paged_evict_select, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return e;
         prepared[dev] = true;
     }
