@@ -117,10 +117,6 @@ __global__ void __launch_bounds__(LG_THREADS, 4) k_logits(const mcpm_logits_para
     for (int c0 = 0, c1; c0 < mine; c0 = c1) {
         c1 = min(mine, c0 + LG_CHUNKS);
         if constexpr (LISTS) {
-            // the first logits come to registers meanwhile, the others to L2
-            load(c0);
-            if (VEC == 4 && tid >= LG_HELD && tid < c1 - c0 && base_of(c0 + tid) + LG_CHUNK <= V)
-                bulk_prefetch_l2(x + base_of(c0 + tid), LG_CHUNK * 4);
             const int lane = tid & 31;
             // the word of a token, if it is in this slice
             auto word_of = [&](int token) -> unsigned {
@@ -172,6 +168,10 @@ __global__ void __launch_bounds__(LG_THREADS, 4) k_logits(const mcpm_logits_para
                         for (int k = 0; k < LG_BATCH; ++k)
                             if (w[k] != ~0u) queue[at + before[k]] = static_cast<uint16_t>(w[k]);
                     }
+                    // The logits come to L2 while the entries are counted; asked for earlier, they held the history
+                    // up for 5 us.
+                    if (VEC == 4 && r0 == 0 && tid < c1 - c0 && base_of(c0 + tid) + LG_CHUNK <= V)
+                        bulk_prefetch_l2(x + base_of(c0 + tid), LG_CHUNK * 4);
                     __syncthreads();
                     const int n = n_queue;
                     for (int i = tid; i < n; i += LG_THREADS) claim(queue[i]);
@@ -196,9 +196,8 @@ __global__ void __launch_bounds__(LG_THREADS, 4) k_logits(const mcpm_logits_para
                 if (again) c1 = c0 + (c1 - c0 + 1) / 2;   // ends: a chunk's tokens fit the list
             }
         }
-        if (!LISTS) load(c0);
         for (int k0 = c0; k0 < c1; k0 += LG_HELD) {
-            if (k0 > c0) load(k0);
+            load(k0);
 #pragma unroll
             for (int k = 0; k < LG_HELD; ++k) {
                 if (k0 + k >= c1) break;
