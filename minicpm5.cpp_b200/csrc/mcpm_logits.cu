@@ -11,7 +11,7 @@
 namespace mcpm {
 namespace {
 
-constexpr int LG_CLUSTER = 8;        // CTAs that share a row
+constexpr int LG_CLUSTER_BITS = 3, LG_WIDE_BITS = 4;   // CTAs that share a row: 8, or 16 where few rows leave SMs idle
 constexpr int LG_THREADS = 256;
 constexpr int LG_CHUNK_BITS = 10, LG_CHUNK = 1 << LG_CHUNK_BITS;   // tokens that go to one CTA in a row, four a thread
 constexpr int LG_CHUNKS = 16;        // chunks whose words a CTA holds at once
@@ -34,7 +34,7 @@ __device__ __forceinline__ void take(Best& a, const Best& b) {
     if (b.v > a.v || (b.v == a.v && b.t < a.t)) a = b;
 }
 
-// A cluster of LG_CLUSTER CTAs per row.  Chunks of the vocabulary go to them in turn: frequent tokens have low
+// A cluster of 8 or 16 CTAs per row.  Chunks of the vocabulary go to them in turn: frequent tokens have low
 // ids, and with contiguous shares the first CTA had half of a long history (64 rows with 4096 tokens each: 35 us).
 // Per LG_SLICE tokens of a CTA: every thread passes over a share of the history and queues the entries that are
 // this CTA's (an eighth: worked on in place they would keep every warp busy for a few lanes).  The queued tokens
@@ -43,7 +43,7 @@ __device__ __forceinline__ void take(Best& a, const Best& b) {
 // largest index is the last entry).  The streaming pass puts the logits of listed tokens aside, and they are
 // computed side by side after it.  A slice with more listed tokens than the list holds is cut in half until
 // they fit.  VEC = 4 where all rows are 16-byte aligned, else 1.
-template <int VEC, bool LISTS, bool MASK>
+template <int VEC, bool LISTS, bool MASK, int bits_cta>
 __global__ void __launch_bounds__(LG_THREADS, 4) k_logits(const mcpm_logits_params p) {
     extern __shared__ __align__(16) uint16_t words[];    // [LG_SLICE] place on the list plus 1; zero: not listed
     __shared__ uint32_t counts[LISTS ? LG_LISTED : 1];   // the counters of the listed tokens
@@ -51,21 +51,22 @@ __global__ void __launch_bounds__(LG_THREADS, 4) k_logits(const mcpm_logits_para
     __shared__ uint16_t list[LISTS ? LG_LISTED : 1];     // their places in the slice
     __shared__ uint16_t queue[LISTS ? LG_QUEUE : 1];
     __shared__ int n_list, n_queue;
-    __shared__ Best warp_best[LG_THREADS / 32], cta_best[LG_CLUSTER];
+    __shared__ Best warp_best[LG_THREADS / 32], cta_best[1 << LG_WIDE_BITS];
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     if (p.argmax) cluster.barrier_arrive();   // waited for before the first write to another CTA's memory
     grid_dep_launch();
     grid_dep_wait();
-    const int tid = threadIdx.x, rank = cluster.block_rank(), row = blockIdx.x / LG_CLUSTER;
+    constexpr int n_cta = 1 << bits_cta;   // CTAs of the row's cluster
+    const int tid = threadIdx.x, rank = cluster.block_rank(), row = blockIdx.x >> bits_cta;
     const int V = p.n_vocab;
     const float* x = p.logits + row * p.logits_stride;
     float* out = p.out + row * p.out_stride;
     const uint32_t* allow = MASK ? p.allow + row * p.allow_stride : nullptr;
     // chunk k of this CTA begins at token base_of(k); a thread's tokens of it are place(0 .. 3) further
-    auto base_of = [&](int k) { return (k * LG_CLUSTER + rank) << LG_CHUNK_BITS; };
+    auto base_of = [&](int k) { return (k << bits_cta | rank) << LG_CHUNK_BITS; };
     auto place = [&](int e) { return VEC == 4 ? 4 * tid + e : e * LG_THREADS + tid; };
-    const int mine = (((V + LG_CHUNK - 1) >> LG_CHUNK_BITS) - rank + LG_CLUSTER - 1) / LG_CLUSTER;   // chunks of this CTA
+    const int mine = (((V + LG_CHUNK - 1) >> LG_CHUNK_BITS) - rank + n_cta - 1) >> bits_cta;   // chunks of this CTA
     Best best{-INFINITY, 0x7fffffff};
     float v[LG_HELD][4];
     uint32_t bits[LG_HELD][VEC == 4 ? 1 : 4];   // the mask words of the thread's tokens
@@ -120,8 +121,8 @@ __global__ void __launch_bounds__(LG_THREADS, 4) k_logits(const mcpm_logits_para
             const int lane = tid & 31;
             // the word of a token, if it is in this slice
             auto word_of = [&](int token) -> unsigned {
-                const unsigned chunk = static_cast<unsigned>(token) >> LG_CHUNK_BITS, k = chunk / LG_CLUSTER - c0;
-                const bool here = chunk % LG_CLUSTER == rank && k < static_cast<unsigned>(c1 - c0) && token < V;   // a negative token's chunk lies beyond
+                const unsigned chunk = static_cast<unsigned>(token) >> LG_CHUNK_BITS, k = (chunk >> bits_cta) - c0;
+                const bool here = (chunk & (n_cta - 1)) == static_cast<unsigned>(rank) && k < static_cast<unsigned>(c1 - c0) && token < V;   // a negative token's chunk lies beyond
                 return here ? k << LG_CHUNK_BITS | (token & (LG_CHUNK - 1)) : ~0u;
             };
             auto claim = [&](unsigned w) {
@@ -268,9 +269,15 @@ __global__ void __launch_bounds__(LG_THREADS, 4) k_logits(const mcpm_logits_para
     if (rank) return;         // only the first CTA waits for the others
     cluster.barrier_wait();
     if (tid == 0) {
-        for (int c = 1; c < LG_CLUSTER; ++c) take(best, cta_best[c]);
+        for (int c = 1; c < n_cta; ++c) take(best, cta_best[c]);
         p.argmax[row] = best.t == 0x7fffffff ? -1 : best.t;
     }
+}
+
+template <int VEC, int BITS>
+auto pick(bool lists, bool mask) -> void (*)(mcpm_logits_params) {
+    return lists ? mask ? k_logits<VEC, true, true, BITS> : k_logits<VEC, true, false, BITS>
+           : mask ? k_logits<VEC, false, true, BITS> : k_logits<VEC, false, false, BITS>;
 }
 
 }  // namespace
@@ -296,22 +303,23 @@ extern "C" mcpm_status mcpm_logits_process(const mcpm_logits_params* params, voi
     if (p.allow && p.allow_stride < mask_words) return MCPM_BAD_ARG;
     auto aligned = [](const float* q, int64_t stride) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0 && stride % 4 == 0; };
     const bool lists = p.hist || p.bias_token, mask = p.allow != nullptr;
-    void (*kernel)(mcpm_logits_params) = aligned(p.logits, p.logits_stride) && aligned(p.out, p.out_stride)
-                                             ? lists ? mask ? k_logits<4, true, true> : k_logits<4, true, false>
-                                               : mask ? k_logits<4, false, true> : k_logits<4, false, false>
-                                             : lists ? mask ? k_logits<1, true, true> : k_logits<1, true, false>
-                                               : mask ? k_logits<1, false, true> : k_logits<1, false, false>;
+    const bool wide = static_cast<long long>(p.n_seq) << LG_WIDE_BITS <= 128;   // 148 SMs
+    const bool vec = aligned(p.logits, p.logits_stride) && aligned(p.out, p.out_stride);
+    void (*kernel)(mcpm_logits_params) = wide ? (vec ? pick<4, LG_WIDE_BITS>(lists, mask) : pick<1, LG_WIDE_BITS>(lists, mask))
+                                              : (vec ? pick<4, LG_CLUSTER_BITS>(lists, mask) : pick<1, LG_CLUSTER_BITS>(lists, mask));
     const size_t smem = lists ? LG_SLICE * sizeof(uint16_t) : 0;
     cudaError_t e = smem ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) : cudaSuccess;
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e == cudaSuccess) {
+        const unsigned cluster = 1u << (wide ? LG_WIDE_BITS : LG_CLUSTER_BITS);
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(static_cast<unsigned>(p.n_seq) * LG_CLUSTER);
+        cfg.gridDim = dim3(static_cast<unsigned>(p.n_seq) * cluster);
         cfg.blockDim = dim3(LG_THREADS);
         cfg.dynamicSmemBytes = smem;
         cfg.stream = static_cast<cudaStream_t>(stream);
         cudaLaunchAttribute attr[2];
         attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = LG_CLUSTER;
+        attr[0].val.clusterDim.x = cluster;
         attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
         attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // every CTA waits before it reads
         attr[1].val.programmaticStreamSerializationAllowed = 1;
