@@ -236,6 +236,20 @@ def test_attention_graph_replay_with_growing_lengths(cuda):
     del t_dev
 
 
+def test_attention_many_sequences(cuda):
+    """More sequences than a CTA has threads, empty ones among them."""
+    lens = [(37 * i) % 90 if i % 5 else 0 for i in range(600)]
+    c = Cache(cuda, "f16", 4, 2, 64, 16, lens, seed=17)
+    check_attention(c, cuda.randn(600, 4 * 64, device="cuda"))
+
+
+@pytest.mark.parametrize("kv,n_head_kv,lens", [("f16", 1, [40000]), ("f32", 2, [30011, 3, 20000]), ("bf16", 1, [9000, 9001])])
+def test_attention_long_splits(cuda, kv, n_head_kv, lens):
+    """Sequences that all CTAs share: several levels of joins, and masses of positions beyond one CTA's reach."""
+    c = Cache(cuda, kv, 8 * n_head_kv, n_head_kv, 128, 64, lens, seed=18)
+    check_attention(c, cuda.randn(len(lens), 8 * n_head_kv * 128, device="cuda"))
+
+
 def test_attention_shared_prefix_pages(cuda):
     """Two sequences whose first pages are the same pages (no mass is kept)."""
     c = Cache(cuda, "f32", 16, 2, 128, 16, [100, 100], seed=13, mass=False)
@@ -425,6 +439,21 @@ def test_evict(cuda, kv, n_head_kv, dim, page, split):
 def test_evict_long(cuda, n, keep):
     c = Cache(cuda, "f16", 2, 1, 64, 64, [n], seed=n, spare=keep // 64 + 2)
     check_evict(c, keep, 3, 33)
+
+
+def test_evict_long_among_many(cuda):
+    """One CTA per (sequence, head), and more positions than it holds keys of."""
+    lens = [40000] + [10] * 74
+    c = Cache(cuda, "f16", 2, 1, 64, 64, lens, seed=31, spare=75 * 16)
+    check_evict(c, 1000, 3, 33)
+
+
+def test_evict_equal_masses(cuda):
+    """All masses equal, in one CTA and in a cluster: the lowest positions stay."""
+    for n in (3000, 70000):
+        c = Cache(cuda, "f16", 2, 1, 64, 64, [n], seed=n, spare=20)
+        c.mass.fill_(0.0)
+        check_evict(c, 1111, 5, 50)
 
 
 @pytest.mark.parametrize("keep,sink,recent", [(1, 0, 0), (1, 1, 0), (1, 0, 1), (64, 32, 32), (64, 0, 64), (300, 0, 0), (320, 5, 5)])

@@ -116,6 +116,15 @@ def test_logits_counts_and_history_bounds(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,hist", [(1, 20000), (9, 20000), (2, 9001), (3, 100000)])
+def test_logits_long_histories(cuda, n, hist):
+    """More entries than one round takes, and more distinct tokens than a slice's list holds."""
+    r = Rows(cuda, n, 130560, hist, 300, True, seed=hist)
+    r.hist[:] = np.random.default_rng(7).integers(0, 130560, r.hist.shape)
+    r.check()
+
+
+@pytest.mark.gpu
 def test_logits_duplicate_and_foreign_biases(cuda):
     r = Rows(cuda, 2, 500, 0, 4094, seed=2)   # most tokens are listed about eight times: the last entry counts
     r.bias_token[0, ::3] = -1
