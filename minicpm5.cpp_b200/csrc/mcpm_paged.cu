@@ -84,11 +84,10 @@ struct EvictArgs {
     int n_keep, n_sink, n_recent;
 };
 
-constexpr int EV_THREADS = 1024, EV_WARPS = EV_THREADS / 32;
 constexpr int EV_MAX_CLUSTER = 16;   // beyond the portable 8: one GPC's SMs
 constexpr int EV_BITS = 11, EV_BINS = 1 << EV_BITS, EV_PASSES = 3;   // digits of 11, 11 and 10 bits, highest first
 constexpr int EV_KEYS = 32768;   // keys a CTA holds in shared memory
-constexpr int EV_RANKED = 512;   // at most EV_THREADS
+constexpr int EV_RANKED = 512;   // at most a CTA's threads
 constexpr int EV_HELD = 8;       // positions a thread reads at once
 constexpr int EV_SMEM = (EV_PASSES * EV_BINS + EV_KEYS) * 4;
 
@@ -104,9 +103,11 @@ __device__ __forceinline__ uint32_t mass_key(float m) {
 // the n_keep-th largest key: per digit a histogram in each CTA, summed over the cluster, and the bin in
 // which the count from above reaches n_keep.  Then every warp counts its positions above and at the
 // threshold, and writes its part of the list in order.  Keys stay in shared memory between the passes.
-__global__ void __launch_bounds__(EV_THREADS, 1) k_paged_evict_select(const PagedGeom g, const EvictArgs a) {
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_paged_evict_select(const PagedGeom g, const EvictArgs a) {
+    constexpr int WARPS = THREADS / 32;
     extern __shared__ __align__(16) uint32_t ev_smem[];
-    __shared__ int groups[EV_PASSES][EV_BINS / 32], warp_gt[EV_WARPS], warp_eq[EV_WARPS], pick[3], n_cand;
+    __shared__ int groups[EV_PASSES][EV_BINS / 32], warp_gt[32], warp_eq[32], pick[3], n_cand;
     __shared__ int2 cta_sum;
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
@@ -129,7 +130,7 @@ __global__ void __launch_bounds__(EV_THREADS, 1) k_paged_evict_select(const Page
         return mass_key(a.mass[g.mass_at(page, slot, kv)]);
     };
     auto key = [&](int i) { return i < EV_KEYS ? keys[i] : read_key(i); };
-    for (int i = tid; i < EV_PASSES * EV_BINS; i += EV_THREADS) hist[i] = 0u;
+    for (int i = tid; i < EV_PASSES * EV_BINS; i += THREADS) hist[i] = 0u;
     __syncthreads();
     // One count, or one for the whole warp where its keys share a bin (protected positions; equal masses).
     auto count = [&](uint32_t* h, int bin) {   // whole warps; bin -1: none
@@ -142,15 +143,15 @@ __global__ void __launch_bounds__(EV_THREADS, 1) k_paged_evict_select(const Page
             atomicAdd(&h[bin], 1u);
         }
     };
-    for (int i0 = 32 * warp; i0 < m; i0 += EV_HELD * EV_THREADS) {   // EV_HELD positions of a thread in flight
-        const int batch = min(EV_HELD, (m - i0 + EV_THREADS - 1) / EV_THREADS);   // of the warp
+    for (int i0 = 32 * warp; i0 < m; i0 += EV_HELD * THREADS) {   // EV_HELD positions of a thread in flight
+        const int batch = min(EV_HELD, (m - i0 + THREADS - 1) / THREADS);   // of the warp
         int page[EV_HELD], slot[EV_HELD];
         float x[EV_HELD];
         bool present[EV_HELD];
 #pragma unroll
         for (int k = 0; k < EV_HELD; ++k)
             if (k < batch) {
-                const int i = i0 + lane + k * EV_THREADS;
+                const int i = i0 + lane + k * THREADS;
                 present[k] = i < m && g.locate(row, lo + i, page[k], slot[k]);
             }
 #pragma unroll
@@ -159,7 +160,7 @@ __global__ void __launch_bounds__(EV_THREADS, 1) k_paged_evict_select(const Page
 #pragma unroll
         for (int k = 0; k < EV_HELD; ++k)
             if (k < batch) {
-                const int i = i0 + lane + k * EV_THREADS, j = lo + i;
+                const int i = i0 + lane + k * THREADS, j = lo + i;
                 const uint32_t y = !present[k] ? 0u : j < a.n_sink || j >= n - a.n_recent ? 0xffffffffu : mass_key(x[k]);
                 if (i < m && i < EV_KEYS) keys[i] = y;
                 count(hist, present[k] ? static_cast<int>(y >> (32 - EV_BITS)) : -1);
@@ -175,13 +176,13 @@ __global__ void __launch_bounds__(EV_THREADS, 1) k_paged_evict_select(const Page
         uint32_t* mine = hist + pass * EV_BINS;
         if (pass > 0) {
             const int above = low + (pass == 1 ? EV_BITS : 32 - 2 * EV_BITS);
-            for (int i0 = 32 * warp; i0 < m; i0 += EV_THREADS) {
+            for (int i0 = 32 * warp; i0 < m; i0 += THREADS) {
                 const uint32_t k = i0 + lane < m ? key(i0 + lane) : 0u;
                 count(mine, k && (k >> above) == (prefix >> above) ? static_cast<int>(k >> low & ((1u << (above - low)) - 1u)) : -1);
             }
         }
         __syncthreads();
-        for (int q = warp; q < EV_BINS / 32; q += EV_WARPS) {
+        for (int q = warp; q < EV_BINS / 32; q += WARPS) {
             const int s = __reduce_add_sync(0xffffffffu, mine[32 * q + lane]);
             if (lane == 0) groups[pass][q] = s;
         }
@@ -227,7 +228,7 @@ __global__ void __launch_bounds__(EV_THREADS, 1) k_paged_evict_select(const Page
             fb += above;
             const unsigned hit = __ballot_sync(0xffffffffu, fb < need && fb + f >= need);
             const int at = hit ? __ffs(hit) - 1 : 31;
-            if (lane == at) pick[0] = 32 * group + 31 - lane, pick[1] = fb, pick[2] = hit ? f : EV_THREADS + 1;
+            if (lane == at) pick[0] = 32 * group + 31 - lane, pick[1] = fb, pick[2] = hit ? f : THREADS + 1;
         }
         __syncthreads();
         prefix |= static_cast<uint32_t>(pick[0]) << low;
@@ -240,7 +241,7 @@ __global__ void __launch_bounds__(EV_THREADS, 1) k_paged_evict_select(const Page
             uint32_t* cand = hist + (pass + 1) * EV_BINS;   // zeroed; this CTA's, then behind EV_RANKED all of them
             if (tid == 0) n_cand = 0;
             __syncthreads();
-            for (int i = tid; i < m; i += EV_THREADS) {
+            for (int i = tid; i < m; i += THREADS) {
                 const uint32_t k = key(i);
                 if (k && (k >> low) == (prefix >> low)) cand[atomicAdd(&n_cand, 1)] = k;
             }
@@ -270,7 +271,7 @@ __global__ void __launch_bounds__(EV_THREADS, 1) k_paged_evict_select(const Page
         }
     }
     // each warp's contiguous positions: how many are above the threshold, how many at it
-    const int per = ((m + EV_WARPS - 1) / EV_WARPS + 31) & ~31;
+    const int per = ((m + WARPS - 1) / WARPS + 31) & ~31;
     const int w0 = min(m, warp * per), w1 = min(m, w0 + per);
     int gt = 0, eq = 0;
     for (int i = w0 + lane; i - lane < w1; i += 32) {
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__(EV_THREADS, 1) k_paged_evict_select(const Page
     if (lane == 0) warp_gt[warp] = gt, warp_eq[warp] = eq;
     __syncthreads();
     // before this warp, and in the whole CTA
-    const int wg = warp_gt[lane], we = warp_eq[lane];
+    const int wg = lane < WARPS ? warp_gt[lane] : 0, we = lane < WARPS ? warp_eq[lane] : 0;
     int g0 = __reduce_add_sync(0xffffffffu, lane < warp ? wg : 0), e0 = __reduce_add_sync(0xffffffffu, lane < warp ? we : 0);
     int g_all = __reduce_add_sync(0xffffffffu, wg), e_all = __reduce_add_sync(0xffffffffu, we);
     if (n_cta > 1) {
@@ -307,7 +308,7 @@ __global__ void __launch_bounds__(EV_THREADS, 1) k_paged_evict_select(const Page
         e0 += __popc(me);
     }
     const int total = g_all + min(e_all, need);
-    for (int i = total + rank * EV_THREADS + tid; i < a.n_keep; i += n_cta * EV_THREADS) kept[i] = -1;
+    for (int i = total + rank * THREADS + tid; i < a.n_keep; i += n_cta * THREADS) kept[i] = -1;
     if (tid == 0 && kv == 0 && rank == 0) a.new_len[seq] = total;
     if (n_cta > 1) cluster.sync();   // no CTA ends while another reads its counts
 }
@@ -360,25 +361,32 @@ cudaError_t launch_evict_copy(const PagedGeom& g, const EvictArgs& a, int n_seq,
     return launch_dependent(g.head_dim == 64 ? k_paged_evict_copy<T, 64> : k_paged_evict_copy<T, 128>, grid, 32 * EV_COPY_WARPS, 0, s, g, a);
 }
 
-// One CTA for up to 4096 positions, more where the table has room for longer sequences and SMs are free.
+// One CTA for up to 4096 positions, more where the table has room for longer sequences and SMs are free; CTAs of
+// 512 threads, two to an SM, where there are more pairs than SMs (200 pairs of 2621 positions: a second wave of
+// selections cost 9 us).
+template <int THREADS>
+cudaError_t prepare_select(int dev) {
+    static bool prepared[64] = {};
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (prepared[dev]) return cudaSuccess;
+    cudaError_t e = cudaFuncSetAttribute(k_paged_evict_select<THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_SMEM);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_paged_evict_select<THREADS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    prepared[dev] = e == cudaSuccess;
+    return e;
+}
 cudaError_t launch_evict_select(const PagedGeom& g, const EvictArgs& a, int n_seq, cudaStream_t s) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    static bool prepared[64] = {};
-    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    if (!prepared[dev]) {
-        e = cudaFuncSetAttribute(k_paged_evict_select, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_SMEM);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(k_paged_evict_select, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e != cudaSuccess) return e;
-        prepared[dev] = true;
-    }
     const long long room = static_cast<long long>(g.max_pages) * g.page_size, pairs = static_cast<long long>(n_seq) * g.n_head_kv;
+    const bool many = pairs > 148;   // SMs
+    e = many ? prepare_select<512>(dev) : prepare_select<1024>(dev);
+    if (e != cudaSuccess) return e;
     int cluster = 1;
-    while (cluster < EV_MAX_CLUSTER && cluster * 4096LL < room && pairs * cluster * 2 <= 148) cluster *= 2;
+    while (cluster < EV_MAX_CLUSTER && cluster * 4096LL < room && pairs * cluster * 2 <= 128) cluster *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(g.n_head_kv * cluster, n_seq);
-    cfg.blockDim = dim3(EV_THREADS);
+    cfg.blockDim = dim3(many ? 512 : 1024);
     const long long keys = std::min<long long>(EV_KEYS, (room + cluster - 1) / cluster + 32);
     cfg.dynamicSmemBytes = (EV_PASSES * EV_BINS + static_cast<size_t>(keys)) * 4;
     cfg.stream = s;
@@ -390,7 +398,7 @@ cudaError_t launch_evict_select(const PagedGeom& g, const EvictArgs& a, int n_se
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    return cudaLaunchKernelEx(&cfg, k_paged_evict_select, g, a);
+    return cudaLaunchKernelEx(&cfg, many ? k_paged_evict_select<512> : k_paged_evict_select<1024>, g, a);
 }
 
 // ---------------------------------------------------------------- host side
