@@ -277,10 +277,24 @@ __global__ void __launch_bounds__(LG_THREADS, 4) k_logits(const mcpm_logits_para
     }
 }
 
+using Kernel = void (*)(mcpm_logits_params);
+
+// The kernel of a variant, its attributes set once per device (setting them again does no harm).
+template <int VEC, int BITS, bool LISTS, bool MASK>
+cudaError_t prepared(int dev, Kernel& kernel) {
+    static bool done[64] = {};
+    kernel = k_logits<VEC, LISTS, MASK, BITS>;
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (done[dev]) return cudaSuccess;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LG_SLICE * static_cast<int>(sizeof(uint16_t)));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    done[dev] = e == cudaSuccess;
+    return e;
+}
 template <int VEC, int BITS>
-auto pick(bool lists, bool mask) -> void (*)(mcpm_logits_params) {
-    return lists ? mask ? k_logits<VEC, true, true, BITS> : k_logits<VEC, true, false, BITS>
-           : mask ? k_logits<VEC, false, true, BITS> : k_logits<VEC, false, false, BITS>;
+cudaError_t pick(bool lists, bool mask, int dev, Kernel& kernel) {
+    return lists ? mask ? prepared<VEC, BITS, true, true>(dev, kernel) : prepared<VEC, BITS, true, false>(dev, kernel)
+           : mask ? prepared<VEC, BITS, false, true>(dev, kernel) : prepared<VEC, BITS, false, false>(dev, kernel);
 }
 
 }  // namespace
@@ -308,11 +322,13 @@ extern "C" mcpm_status mcpm_logits_process(const mcpm_logits_params* params, voi
     const bool lists = p.hist || p.bias_token, mask = p.allow != nullptr;
     const bool wide = static_cast<long long>(p.n_seq) << LG_WIDE_BITS <= 128;   // 148 SMs
     const bool vec = aligned(p.logits, p.logits_stride) && aligned(p.out, p.out_stride);
-    void (*kernel)(mcpm_logits_params) = wide ? (vec ? pick<4, LG_WIDE_BITS>(lists, mask) : pick<1, LG_WIDE_BITS>(lists, mask))
-                                              : (vec ? pick<4, LG_CLUSTER_BITS>(lists, mask) : pick<1, LG_CLUSTER_BITS>(lists, mask));
     const size_t smem = lists ? LG_SLICE * sizeof(uint16_t) : 0;
-    cudaError_t e = smem ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) : cudaSuccess;
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    int dev = 0;
+    Kernel kernel = nullptr;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess)
+        e = wide ? (vec ? pick<4, LG_WIDE_BITS>(lists, mask, dev, kernel) : pick<1, LG_WIDE_BITS>(lists, mask, dev, kernel))
+                 : (vec ? pick<4, LG_CLUSTER_BITS>(lists, mask, dev, kernel) : pick<1, LG_CLUSTER_BITS>(lists, mask, dev, kernel));
     if (e == cudaSuccess) {
         const unsigned cluster = 1u << (wide ? LG_WIDE_BITS : LG_CLUSTER_BITS);
         cudaLaunchConfig_t cfg = {};
