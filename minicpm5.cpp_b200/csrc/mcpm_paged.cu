@@ -90,7 +90,7 @@ constexpr int EV_MAX_CLUSTER = 16;   // beyond the portable 8: one GPC's SMs
 constexpr int EV_BITS = 11, EV_BINS = 1 << EV_BITS, EV_PASSES = 3;   // digits of 11, 11 and 10 bits, highest first
 constexpr int EV_KEYS = 32768;   // keys a CTA holds in shared memory
 constexpr int EV_RANKED = 512;   // at most a CTA's threads
-constexpr int EV_HELD = 8;       // positions a thread reads at once
+constexpr int EV_HELD = 4;       // positions a thread reads at once
 constexpr int EV_SMEM = (EV_PASSES * EV_BINS + EV_KEYS) * 4;
 
 // Order-preserving unsigned key of a position: a larger key is kept first.  Absent positions 0, NaN 1
@@ -265,7 +265,12 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) k_paged_evict_select(
             if (tid < in_bin) {
                 const uint32_t k = all[tid];
                 int above = 0, at = 0;
-                for (int i = 0; i < in_bin; ++i) above += all[i] > k, at += all[i] == k;
+#pragma unroll 4
+                for (int i = 0; i < in_bin; i += 4) {   // the list ends in zeros, which are no keys
+                    const uint4 x = *reinterpret_cast<const uint4*>(all + i);
+                    above += (x.x > k) + (x.y > k) + (x.z > k) + (x.w > k);
+                    at += (x.x == k) + (x.y == k) + (x.z == k) + (x.w == k);
+                }
                 if (above < need && above + at >= need) pick[1] = static_cast<int>(k), pick[2] = need - above;   // equal keys write the same
             }
             __syncthreads();
