@@ -318,7 +318,7 @@ extern "C" mcpm_status mcpm_logits_process(const mcpm_logits_params* params, voi
     if (p.hist && (!p.penalties || p.hist_max < 0 || p.hist_max > LG_MAX_HIST || p.hist_stride < p.hist_max)) return MCPM_BAD_ARG;
     if (p.bias_token && (!p.bias || p.bias_max < 0 || p.bias_max > LG_MAX_BIAS || p.bias_stride < p.bias_max)) return MCPM_BAD_ARG;
     if (p.allow && p.allow_stride < mask_words) return MCPM_BAD_ARG;
-    auto aligned = [](const float* q, int64_t stride) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0 && stride % 4 == 0; };
+    auto aligned = [&](const float* q, int64_t stride) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0 && (p.n_seq == 1 || stride % 4 == 0); };
     const bool lists = p.hist || p.bias_token, mask = p.allow != nullptr;
     const bool wide = static_cast<long long>(p.n_seq) << LG_WIDE_BITS <= 128;   // 148 SMs
     const bool vec = aligned(p.logits, p.logits_stride) && aligned(p.out, p.out_stride);

@@ -19,8 +19,8 @@
 //
 // Measured (16 query heads, 2 KV heads, 128 dims): 4 x 131072 positions of fp16 93 us, 5.8 TB/s; of fp32 171 us,
 // 6.3 TB/s; bound by the memory (a device copy: 6.46 TB/s).  Short calls are bound by a chain of round trips:
-// lengths, page table, K, V, then record, arrival and join where a pair is split: 8193 fp32 positions 13.5 us,
-// of which 2.6 us are bytes; 137 positions 8.6 us.
+// lengths, page table, K, V, then record, arrival and join where a pair is split: 8193 fp32 positions 13.7 us,
+// of which 2.6 us are bytes; 137 positions 8.7 us.
 #include <algorithm>
 #include <cmath>
 
@@ -39,7 +39,7 @@ constexpr int FAN = 16, FAN_BITS = 4, LEVELS = 3;   // records joined at a time,
 // units (q, the join of the warps, the output).  An end of a share inside a pair of at most WHOLE units, among its
 // LEAD steps or within `slack` units of one of its ends moves to that end: the rest would cost more as a record
 // with its arrival and join than as work.
-constexpr int WHOLE = 2, LEAD = 2;
+constexpr int WHOLE = 2, LEAD = 1;   // LEAD 1, 2, 3: 30.6, 31.6, 32.8 us at 200 sequences of 20 to 900 fp16 positions
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float P_SCALE = 1024.0f;  // weights are multiplied by this before they are split: fp16 parts of small
                                     // weights stay normal; undone in the output
