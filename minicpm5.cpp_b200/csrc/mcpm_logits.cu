@@ -14,15 +14,20 @@ namespace {
 constexpr int LG_CLUSTER_BITS = 3, LG_WIDE_BITS = 4;   // CTAs that share a row: 8, or 16 where few rows leave SMs idle
 constexpr int LG_THREADS = 256;
 constexpr int LG_CHUNK_BITS = 10, LG_CHUNK = 1 << LG_CHUNK_BITS;   // tokens that go to one CTA in a row, four a thread
-constexpr int LG_CHUNKS = 16;        // chunks whose words a CTA holds at once
-constexpr int LG_SLICE = LG_CHUNKS * LG_CHUNK;
+constexpr int LG_CHUNKS = 32;        // most chunks whose words a CTA holds at once (places are 16 bits)
 constexpr int LG_HELD = 4;           // chunks in registers at once
 constexpr int LG_BATCH = 8;          // history entries of a thread in flight
 constexpr int LG_QUEUE = 2 * LG_BATCH * LG_THREADS;   // history entries of a CTA in one round
 constexpr int LG_LISTED = 1024;      // listed tokens of a slice
 constexpr int LG_COUNT_BITS = 20;    // counter: times in the history; above: last bias entry + 1
 constexpr int LG_MAX_HIST = (1 << LG_COUNT_BITS) - 1, LG_MAX_BIAS = (1 << (32 - LG_COUNT_BITS)) - 2;
-static_assert(LG_CHUNK == 4 * LG_THREADS && LG_SLICE <= 32768 && LG_CHUNKS % LG_HELD == 0, "");
+static_assert(LG_CHUNK == 4 * LG_THREADS && LG_CHUNKS * LG_CHUNK <= 65536 && LG_CHUNKS % LG_HELD == 0, "");
+// Chunks of a CTA's slice: all of them where they fit, since each slice passes over the history again (39 rows of
+// 161648 with histories of 3180: two slices 26 us, one 19 us).
+__host__ __device__ inline int slice_chunks(int n_vocab, int bits_cta) {
+    const int mine = (((n_vocab - 1) >> LG_CHUNK_BITS) >> bits_cta) + 1;
+    return mine < LG_CHUNKS ? mine : LG_CHUNKS;
+}
 static_assert(LG_LISTED >= LG_CHUNK, "one chunk's tokens fit the list");
 
 struct Best {
@@ -36,7 +41,7 @@ __device__ __forceinline__ void take(Best& a, const Best& b) {
 
 // A cluster of 8 or 16 CTAs per row.  Chunks of the vocabulary go to them in turn: frequent tokens have low
 // ids, and with contiguous shares the first CTA had half of a long history (64 rows with 4096 tokens each: 35 us).
-// Per LG_SLICE tokens of a CTA: every thread passes over a share of the history and queues the entries that are
+// Per slice of a CTA's tokens: every thread passes over a share of the history and queues the entries that are
 // this CTA's (an eighth: worked on in place they would keep every warp busy for a few lanes).  The queued tokens
 // claim their 16-bit words, the first of each takes a place on a list, and then every entry counts at its
 // token's place and every bias entry leaves its index there (integer atomics: the order does not matter; the
@@ -48,7 +53,7 @@ __device__ __forceinline__ void take(Best& a, const Best& b) {
 // One row 6.5 us.
 template <int VEC, bool LISTS, bool MASK, int bits_cta>
 __global__ void __launch_bounds__(LG_THREADS, 4) k_logits(const mcpm_logits_params p) {
-    extern __shared__ __align__(16) uint16_t words[];    // [LG_SLICE] place on the list plus 1; zero: not listed
+    extern __shared__ __align__(16) uint16_t words[];    // [tokens of a slice] place on the list plus 1; zero: not listed
     __shared__ uint32_t counts[LISTS ? LG_LISTED : 1];   // the counters of the listed tokens
     __shared__ float aside[LISTS ? LG_LISTED : 1];       // their logits
     __shared__ uint16_t list[LISTS ? LG_LISTED : 1];     // their places in the slice
@@ -119,7 +124,7 @@ __global__ void __launch_bounds__(LG_THREADS, 4) k_logits(const mcpm_logits_para
         return b ? __fadd_rn(y, p.bias[row * p.bias_stride + b - 1]) : y;
     };
     for (int c0 = 0, c1; c0 < mine; c0 = c1) {
-        c1 = min(mine, c0 + LG_CHUNKS);
+        c1 = min(mine, c0 + slice_chunks(V, bits_cta));
         if constexpr (LISTS) {
             const int lane = tid & 31;
             // the word of a token, if it is in this slice
@@ -286,7 +291,7 @@ cudaError_t prepared(int dev, Kernel& kernel) {
     kernel = k_logits<VEC, LISTS, MASK, BITS>;
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
     if (done[dev]) return cudaSuccess;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LG_SLICE * static_cast<int>(sizeof(uint16_t)));
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LG_CHUNKS * LG_CHUNK * static_cast<int>(sizeof(uint16_t)));
     if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     done[dev] = e == cudaSuccess;
     return e;
@@ -322,7 +327,8 @@ extern "C" mcpm_status mcpm_logits_process(const mcpm_logits_params* params, voi
     const bool lists = p.hist || p.bias_token, mask = p.allow != nullptr;
     const bool wide = static_cast<long long>(p.n_seq) << LG_WIDE_BITS <= 128;   // 148 SMs
     const bool vec = aligned(p.logits, p.logits_stride) && aligned(p.out, p.out_stride);
-    const size_t smem = lists ? LG_SLICE * sizeof(uint16_t) : 0;
+    const int bits_cta = wide ? LG_WIDE_BITS : LG_CLUSTER_BITS;
+    const size_t smem = lists ? slice_chunks(p.n_vocab, bits_cta) * LG_CHUNK * sizeof(uint16_t) : 0;
     int dev = 0;
     Kernel kernel = nullptr;
     cudaError_t e = cudaGetDevice(&dev);
@@ -330,7 +336,7 @@ extern "C" mcpm_status mcpm_logits_process(const mcpm_logits_params* params, voi
         e = wide ? (vec ? pick<4, LG_WIDE_BITS>(lists, mask, dev, kernel) : pick<1, LG_WIDE_BITS>(lists, mask, dev, kernel))
                  : (vec ? pick<4, LG_CLUSTER_BITS>(lists, mask, dev, kernel) : pick<1, LG_CLUSTER_BITS>(lists, mask, dev, kernel));
     if (e == cudaSuccess) {
-        const unsigned cluster = 1u << (wide ? LG_WIDE_BITS : LG_CLUSTER_BITS);
+        const unsigned cluster = 1u << bits_cta;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3(static_cast<unsigned>(p.n_seq) * cluster);
         cfg.blockDim = dim3(LG_THREADS);

@@ -116,6 +116,13 @@ def test_logits_counts_and_history_bounds(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,v", [(1, 600001), (9, 300007), (9, 524288)])
+def test_logits_large_vocabularies(cuda, n, v):
+    """Shares of a CTA beyond one slice."""
+    Rows(cuda, n, v, 900, 50, True, seed=v).check()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("n,hist", [(1, 20000), (9, 20000), (2, 9001), (3, 100000)])
 def test_logits_long_histories(cuda, n, hist):
     """More entries than one round takes, and more distinct tokens than a slice's list holds."""
