@@ -371,7 +371,8 @@ cudaError_t launch_evict_copy(const PagedGeom& g, const EvictArgs& a, int n_seq,
     return launch_dependent(g.head_dim == 64 ? k_paged_evict_copy<T, 64> : k_paged_evict_copy<T, 128>, grid, 32 * EV_COPY_WARPS, 0, s, g, a);
 }
 
-// One CTA for up to 4096 positions, more where the table has room for longer sequences and SMs are free; CTAs of
+// One CTA for up to 3072 positions, more where the table has room for longer sequences and SMs are free (8000
+// positions: one CTA 16.6 us with the copy, two 15.5, four 13.3; 2112: one 11.4, two 12.3); CTAs of
 // 512 threads, two to an SM, where there are more pairs than SMs (200 pairs of 2621 positions: a second wave of
 // selections cost 9 us).
 template <int THREADS>
@@ -393,7 +394,7 @@ cudaError_t launch_evict_select(const PagedGeom& g, const EvictArgs& a, int n_se
     e = many ? prepare_select<512>(dev) : prepare_select<1024>(dev);
     if (e != cudaSuccess) return e;
     int cluster = 1;
-    while (cluster < EV_MAX_CLUSTER && cluster * 4096LL < room && pairs * cluster * 2 <= 128) cluster *= 2;
+    while (cluster < EV_MAX_CLUSTER && cluster * 3072LL < room && pairs * cluster * 2 <= 128) cluster *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(g.n_head_kv * cluster, n_seq);
     cfg.blockDim = dim3(many ? 512 : 1024);
