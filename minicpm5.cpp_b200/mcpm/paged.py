@@ -132,6 +132,37 @@ class PagedDecoder:
         return torch.cuda.current_stream().cuda_stream
 
     # ---------------------------------------------------------------- one step
+    def _needs_page(self, seq: int, length: int) -> bool:
+        return length % self.page_size == 0 and self.table[seq, length // self.page_size] < 0
+
+    def _check(self, tokens: Dict[int, int]) -> List[int]:
+        """Raises where a step of these tokens cannot be made, before anything has changed; else the sequences that it
+        evicts.  Pages are counted in the step's own order: an eviction takes its fresh ones before it frees the old."""
+        evicted, free = [], len(self.free)
+        for s, token in tokens.items():
+            if not self.opened[s] or not 0 <= token < self.n_vocab:
+                raise E.MCPMError(E.BAD_TOKEN if self.opened[s] else E.BAD_ARG, f"sequence {s}")
+            length, fresh = int(self.length[s]), 0
+            if self.keep and length >= self.keep + self.slack:
+                evicted.append(s)
+                fresh, length = -(-self.keep // self.page_size), self.keep
+            if length >= self.max_positions or self.position[s] >= self.rope.shape[0]:
+                raise E.MCPMError(E.CTX_OVERFLOW, f"sequence {s}")
+            more = length % self.page_size == 0 if fresh else self._needs_page(s, length)
+            held = int((self.table[s] >= 0).sum()) if fresh else 0
+            if free < fresh or free - fresh + held < more:
+                raise E.MCPMError(E.OOM, f"page pool exhausted, sequence {s}")
+            free += held - fresh - more
+        return evicted
+
+    def _admit(self, seqs: List[int], evicted: List[int]) -> None:
+        """Makes room for one more position of each sequence, as _check has found possible."""
+        for s in seqs:
+            if s in evicted:
+                self._evict(s)
+            if self._needs_page(s, self.length[s]):
+                self.table[s, self.length[s] // self.page_size] = self._take(1)[0]
+
     def _gemv(self, name: str, xq: torch.Tensor, out_ptr: int) -> None:
         t = self.tensors[name]
         E.gemv_q8k_block(t.ggml_type, self.weights[name].data_ptr(), xq.data_ptr(), out_ptr, t.dims[1], t.dims[0], self._stream())
@@ -142,15 +173,7 @@ class PagedDecoder:
         Penalties count the tokens fed so far; allow: bool [n_vocab] or [len(tokens)][n_vocab]."""
         seqs = list(tokens)
         n = len(seqs)
-        for s in seqs:
-            if not self.opened[s] or not 0 <= tokens[s] < self.n_vocab:
-                raise E.MCPMError(E.BAD_TOKEN if self.opened[s] else E.BAD_ARG, f"sequence {s}")
-            if self.keep and self.length[s] >= self.keep + self.slack:
-                self._evict(s)
-            if self.length[s] >= self.max_positions or self.position[s] >= self.rope.shape[0]:
-                raise E.MCPMError(E.CTX_OVERFLOW, f"sequence {s}")
-            if self.length[s] % self.page_size == 0:
-                self.table[s, self.length[s] // self.page_size] = self._take(1)[0]
+        self._admit(seqs, self._check(tokens))
         st, ws = self._stream(), (self.workspace.data_ptr(), self.workspace.numel())
         table, slot = self._dev(self.table[seqs]), self._dev(self.length[seqs])
         pos, length = self._dev(self.position[seqs]), self._dev(self.length[seqs] + 1)

@@ -184,3 +184,36 @@ def test_paged_decoder_refusals(cuda, parity):
     with pytest.raises(E.MCPMError) as e:   # the only page is full
         d.step({s: 1})
     assert e.value.status == E.OOM
+
+
+@pytest.mark.gpu
+def test_a_refused_step_can_be_repeated(cuda, parity):
+    """Two sequences at the end of their first page, a bad token and a pool without room: nothing is taken or lost,
+    the step made good writes what an undisturbed one writes, and every page comes back."""
+    from mcpm import engine as E, paged, synth
+    _, _, path = parity
+    ids = [[int(t) for t in synth.prompt_ids(17, seed=s)] for s in (4, 5)]
+
+    def start(n_pages):
+        d = paged.PagedDecoder(path, n_pages=n_pages, max_positions=32, max_seqs=3)
+        a, b = d.open(), d.open()
+        for t in range(16):
+            d.step({a: ids[0][t], b: ids[1][t]})
+        return d, a, b
+
+    d, a, b = start(4)
+    want = d.step({a: ids[0][16], b: ids[1][16]}), _rows(d, a), _rows(d, b)
+    d, a, b = start(4)
+    c = d.open()
+    d.step({c: 1})
+    for status, tokens in ((E.BAD_TOKEN, {a: ids[0][16], b: -1}), (E.OOM, {a: ids[0][16], b: ids[1][16]})):
+        for _ in range(3):
+            with pytest.raises(E.MCPMError) as e:
+                d.step(tokens)
+            assert e.value.status == status and len(d.free) == 1 and d.length[a] == d.length[b] == 16
+    d.close(c)
+    assert d.step({a: ids[0][16], b: ids[1][16]}) == want[0]
+    for got, rows in ((_rows(d, a), want[1]), (_rows(d, b), want[2])):
+        assert np.array_equal(got[0], rows[0]) and np.array_equal(got[1], rows[1])
+    d.close(a), d.close(b)
+    assert sorted(d.free) == list(range(4))

@@ -1,0 +1,105 @@
+"""The paged decoder's host side: which steps it refuses, and that a refused step leaves sequences and pages as they
+were.  No GPU: every step here is refused before it reaches the device."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")   # mcpm.paged imports it
+
+
+def decoder(n_pages, max_seqs, lengths, page_size=16, max_positions=64, n_vocab=1000, rope_len=256, **budget):
+    """A decoder without weights whose sequences hold the given numbers of positions."""
+    from mcpm import paged
+    d = paged.PagedDecoder.__new__(paged.PagedDecoder)
+    d.page_size, d.max_seqs, d.max_positions, d.n_vocab = page_size, max_seqs, max_positions, n_vocab
+    d.keep, d.slack, d.sink, d.recent = (budget.get(k, v) for k, v in dict(keep=0, slack=16, sink=4, recent=16).items())
+    d.rope = np.zeros((rope_len, 64, 2), np.float32)
+    d.free = list(range(n_pages))[::-1]
+    d.table = np.full((max_seqs, max_positions // page_size), -1, np.int32)
+    d.length, d.position = np.zeros(max_seqs, np.int32), np.zeros(max_seqs, np.int32)
+    d.opened, d.history = [False] * max_seqs, [[] for _ in range(max_seqs)]
+    d.evictions = []
+    for n in lengths:
+        s = d.open()
+        for c in range(-(-n // page_size)):
+            d.table[s, c] = d._take(1)[0]
+        d.length[s] = d.position[s] = n
+        d.history[s] = list(range(n))
+
+    def evict(seq):   # what _evict does to the pages
+        fresh = np.full(d.table.shape[1], -1, np.int32)
+        pages = d._take(-(-d.keep // d.page_size))
+        fresh[:len(pages)] = pages
+        d._give_back(seq)
+        d.table[seq], d.length[seq] = fresh, d.keep
+        d.evictions.append(seq)
+
+    d._evict = evict
+    return d
+
+
+def state(d):
+    return sorted(d.free), d.table.tolist(), d.length.tolist(), d.position.tolist(), [list(h) for h in d.history], list(d.opened)
+
+
+def refused(d, status, tokens, **options):
+    from mcpm import engine as E
+    before = state(d)
+    with pytest.raises(E.MCPMError) as e:
+        d.step(tokens, **options)
+    assert e.value.status == status
+    assert state(d) == before and not d.evictions
+
+
+def all_pages(d, n_pages):
+    for s in range(d.max_seqs):
+        d.close(s)
+    return sorted(d.free) == list(range(n_pages))
+
+
+def test_a_refused_step_keeps_no_pages():
+    """Two sequences at the end of their pages: whatever stops the second takes no page for the first."""
+    from mcpm import engine as E
+    d = decoder(5, 2, [16, 32])
+    refused(d, E.BAD_TOKEN, {0: 1, 1: 1000})
+    refused(d, E.BAD_TOKEN, {0: 1, 1: -1})
+    d.opened[1] = False
+    refused(d, E.BAD_ARG, {0: 1, 1: 1})
+    d.opened[1] = True
+    d.length[1] = 64
+    refused(d, E.CTX_OVERFLOW, {0: 1, 1: 1})
+    d.length[1] = 32
+    d.free = d.free[:1]   # one page for two
+    refused(d, E.OOM, {0: 1, 1: 1})
+    refused(d, E.OOM, {1: 1, 0: 1})
+    d.table[1, 2] = d._take(1)[0]   # a page that is there is not taken again
+    refused(d, E.OOM, {1: 1, 0: 1})
+
+
+def test_a_refused_step_evicts_nothing():
+    from mcpm import engine as E
+    d = decoder(6, 2, [48, 16], keep=32)
+    refused(d, E.BAD_TOKEN, {0: 1, 1: 1000})
+    d.free = d.free[:1]   # the eviction needs two
+    refused(d, E.OOM, {0: 1})
+    refused(d, E.OOM, {1: 1, 0: 1})
+
+
+@pytest.mark.parametrize("order", [(0, 1, 2), (2, 1, 0), (1, 2, 0)])
+@pytest.mark.parametrize("free", range(8))
+def test_pages_are_counted_in_the_order_of_the_step(order, free):
+    """Evictions give pages back that later sequences of the step may take: what _check admits can be carried out, and
+    what it refuses cannot."""
+    from mcpm import engine as E
+    d = decoder(8 + free, 3, [48, 48, 32], keep=32, recent=8)
+    other = decoder(8 + free, 3, [48, 48, 32], keep=32, recent=8)
+
+    try:
+        evicted = d._check({s: 1 for s in order})
+    except E.MCPMError as e:
+        assert e.status == E.OOM
+        with pytest.raises(E.MCPMError):
+            other._admit(order, [0, 1])
+        return
+    assert evicted == [s for s in order if s < 2]
+    d._admit(order, evicted)
+    assert d.evictions == evicted and all_pages(d, 8 + free)
