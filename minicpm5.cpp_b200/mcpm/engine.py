@@ -406,6 +406,9 @@ def attention(q_ptr, k_ptr, v_ptr, kc_ptr, vc_ptr, pos, max_seq, out_ptr, out_q8
 
 
 # ------------------------------------------------------------------ paged KV cache and logits (device pointers)
+MAX_HIST, MAX_BIAS = 1048575, 4094   # most entries of a row's history and biases in logits_process
+
+
 def paged_config(kv_type: int, n_head: int, n_head_kv: int, head_dim: int, page_size: int, n_pages: int, max_seqs: int,
                  max_pages: int, page_stride: int = 0, row_stride: int = 0, head_stride: int = 0) -> mcpm_paged_config:
     """Geometry of a paged pool: strides in elements, all 0 for packed [page][slot][kv head][dim]."""

@@ -16,8 +16,9 @@ one length there is the engine's batched decode; this is the path for sequences 
 from __future__ import annotations
 
 import argparse
+import operator
 import time
-from typing import Dict, List, Optional
+from typing import Dict, List, Optional, Tuple
 
 import numpy as np
 import torch
@@ -109,8 +110,8 @@ class PagedDecoder:
         self.free += [int(p) for p in self.table[seq] if p >= 0]
         self.table[seq] = -1
 
-    def _dev(self, a: np.ndarray) -> torch.Tensor:
-        return torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32)).cuda()
+    def _dev(self, a: np.ndarray, dtype=np.int32) -> torch.Tensor:
+        return torch.from_numpy(np.ascontiguousarray(a, dtype=dtype)).cuda()
 
     def _evict(self, seq: int) -> None:
         """The sequence's self.keep heaviest positions of each layer and head, on fresh pages."""
@@ -140,7 +141,7 @@ class PagedDecoder:
         evicts.  Pages are counted in the step's own order: an eviction takes its fresh ones before it frees the old."""
         evicted, free = [], len(self.free)
         for s, token in tokens.items():
-            if not self.opened[s] or not 0 <= token < self.n_vocab:
+            if not self.opened[s] or not 0 <= operator.index(token) < self.n_vocab:
                 raise E.MCPMError(E.BAD_TOKEN if self.opened[s] else E.BAD_ARG, f"sequence {s}")
             length, fresh = int(self.length[s]), 0
             if self.keep and length >= self.keep + self.slack:
@@ -163,6 +164,33 @@ class PagedDecoder:
             if self._needs_page(s, self.length[s]):
                 self.table[s, self.length[s] // self.page_size] = self._take(1)[0]
 
+    def _options(self, tokens: Dict[int, int], repetition: float, frequency: float, presence: float,
+                 bias: Optional[Dict[int, float]], allow: Optional[np.ndarray]) -> Tuple[List[torch.Tensor], Dict[str, int]]:
+        """The lists and masks of a step's logits on the device, and the arguments that name them.  Raises where they
+        cannot be made, so that what is wrong with them is found before the step begins."""
+        n, held, more = len(tokens), [], {}
+        if (repetition, frequency, presence) != (1.0, 0.0, 0.0):
+            if not repetition > 0:
+                raise E.MCPMError(E.BAD_ARG, "repetition > 0")
+            rows = [self.history[s] + [t] for s, t in tokens.items()]
+            hist = np.full((n, max(map(len, rows))), -1, np.int32)
+            for r, row in enumerate(rows):
+                hist[r, :len(row)] = row
+            held += [self._dev(hist), self._dev(np.tile(np.array([repetition, frequency, presence]), (n, 1)), np.float32)]
+            more.update(hist=held[0].data_ptr(), hist_stride=hist.shape[1], penalties=held[1].data_ptr())
+        if bias:
+            if len(bias) > E.MAX_BIAS:
+                raise E.MCPMError(E.BAD_ARG, f"more than {E.MAX_BIAS} biases")
+            ids = np.array([t if 0 <= t < self.n_vocab else -1 for t in bias])   # foreign ids are ignored
+            held += [self._dev(np.tile(ids, (n, 1))), self._dev(np.tile(np.array(list(bias.values())), (n, 1)), np.float32)]
+            more.update(bias_token=held[-2].data_ptr(), bias=held[-1].data_ptr(), bias_stride=len(bias))
+        if allow is not None:
+            words = np.zeros((n, (self.n_vocab + 31) // 32 * 32), bool)
+            words[:, :self.n_vocab] = allow
+            held.append(self._dev(np.packbits(words, axis=1, bitorder="little").view(np.int32)))
+            more.update(allow=held[-1].data_ptr())
+        return held, more
+
     def _gemv(self, name: str, xq: torch.Tensor, out_ptr: int) -> None:
         t = self.tensors[name]
         E.gemv_q8k_block(t.ggml_type, self.weights[name].data_ptr(), xq.data_ptr(), out_ptr, t.dims[1], t.dims[0], self._stream())
@@ -173,7 +201,9 @@ class PagedDecoder:
         Penalties count the tokens fed so far; allow: bool [n_vocab] or [len(tokens)][n_vocab]."""
         seqs = list(tokens)
         n = len(seqs)
-        self._admit(seqs, self._check(tokens))
+        evicted = self._check(tokens)
+        held, more = self._options(tokens, repetition, frequency, presence, bias, allow)   # held: the lists' memory
+        self._admit(seqs, evicted)
         st, ws = self._stream(), (self.workspace.data_ptr(), self.workspace.numel())
         table, slot = self._dev(self.table[seqs]), self._dev(self.length[seqs])
         pos, length = self._dev(self.position[seqs]), self._dev(self.length[seqs] + 1)
@@ -209,23 +239,6 @@ class PagedDecoder:
             self.length[s] += 1
             self.position[s] += 1
             self.history[s].append(tokens[s])
-        held = []   # keeps the lists' memory until the call below has been queued
-        more = {}
-        if (repetition, frequency, presence) != (1.0, 0.0, 0.0):
-            most = max(len(self.history[s]) for s in seqs)
-            hist = np.full((n, most), -1, np.int32)
-            for r, s in enumerate(seqs):
-                hist[r, :len(self.history[s])] = self.history[s]
-            held += [self._dev(hist), torch.tensor([[repetition, frequency, presence]] * n, dtype=torch.float32).cuda()]
-            more.update(hist=held[0].data_ptr(), hist_stride=most, penalties=held[1].data_ptr())
-        if bias:
-            held += [self._dev(np.tile(np.array(list(bias)), (n, 1))), torch.tensor([list(bias.values())] * n, dtype=torch.float32).cuda()]
-            more.update(bias_token=held[-2].data_ptr(), bias=held[-1].data_ptr(), bias_stride=len(bias))
-        if allow is not None:
-            words = np.zeros((n, (self.n_vocab + 31) // 32 * 32), bool)
-            words[:, :self.n_vocab] = allow
-            held.append(self._dev(np.packbits(words, axis=1, bitorder="little").view(np.int32)))
-            more.update(allow=held[-1].data_ptr())
         E.logits_process(self.logits.data_ptr(), self.processed.data_ptr(), n, self.n_vocab, argmax=self.token.data_ptr(), stream=st, **more)
         return dict(zip(seqs, self.token[:n].tolist()))
 

@@ -217,3 +217,28 @@ def test_a_refused_step_can_be_repeated(cuda, parity):
         assert np.array_equal(got[0], rows[0]) and np.array_equal(got[1], rows[1])
     d.close(a), d.close(b)
     assert sorted(d.free) == list(range(4))
+
+
+@pytest.mark.gpu
+def test_a_refused_option_can_be_corrected(cuda, parity):
+    """A step whose mask or biases are refused feeds nothing: the corrected one is the undisturbed one."""
+    from mcpm import engine as E, paged, synth
+    _, _, path = parity
+    ids = [int(t) for t in synth.prompt_ids(6, seed=11)]
+    options = dict(repetition=1.3, frequency=0.2, presence=0.1, bias={7: 2.0, 130560: 9.0, 2 ** 40: 9.0, -3: 9.0}, allow=np.arange(130560) % 3 > 0)
+
+    def run(disturb):
+        d = paged.PagedDecoder(path, n_pages=4, max_positions=32)
+        s, out = d.open(), []
+        for t in ids:
+            if disturb:
+                with pytest.raises(ValueError):
+                    d.step({s: t}, **{**options, "allow": np.ones(5, bool)})
+                with pytest.raises(E.MCPMError):
+                    d.step({s: t}, **{**options, "bias": dict.fromkeys(range(5000), 0.0)})
+            out.append(d.step({s: t}, **options)[s])
+        assert d.history[s] == ids and d.length[s] == d.position[s] == len(ids)
+        return out, d.processed[0].cpu().numpy()
+
+    a, b = run(False), run(True)
+    assert a[0] == b[0] and np.array_equal(a[1], b[1])

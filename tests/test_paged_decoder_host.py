@@ -42,11 +42,12 @@ def state(d):
 
 
 def refused(d, status, tokens, **options):
+    """status: of an MCPMError, or the exception's type."""
     from mcpm import engine as E
     before = state(d)
-    with pytest.raises(E.MCPMError) as e:
+    with pytest.raises(status if isinstance(status, type) else E.MCPMError) as e:
         d.step(tokens, **options)
-    assert e.value.status == status
+    assert isinstance(status, type) or e.value.status == status
     assert state(d) == before and not d.evictions
 
 
@@ -103,3 +104,24 @@ def test_pages_are_counted_in_the_order_of_the_step(order, free):
     assert evicted == [s for s in order if s < 2]
     d._admit(order, evicted)
     assert d.evictions == evicted and all_pages(d, 8 + free)
+
+
+def test_a_refused_option_feeds_no_token():
+    """Masks of the wrong shape, too many biases and penalties that mean nothing are found before the step begins."""
+    from mcpm import engine as E
+    d = decoder(6, 2, [48, 16], keep=32)
+    t = {0: 1, 1: 2}
+    refused(d, ValueError, t, allow=np.ones(999, bool))
+    refused(d, ValueError, t, allow=np.ones((3, 1000), bool))
+    refused(d, E.BAD_ARG, t, bias={i: 1.0 for i in range(E.MAX_BIAS + 1)})
+    for r in (0.0, -1.0, float("nan")):
+        refused(d, E.BAD_ARG, t, repetition=r)
+    refused(d, TypeError, {0: 1, 1: 2.5})
+
+
+def test_limits_are_the_operators_own():
+    from mcpm import engine as E
+    lib = E.load_library()
+    for more in (dict(hist=256, penalties=256, hist_max=E.MAX_HIST + 1), dict(bias_token=256, bias=256, bias_max=E.MAX_BIAS + 1)):
+        p = E.mcpm_logits_params(n_seq=1, n_vocab=100, logits=256, out=512, **more)
+        assert lib.mcpm_logits_process(p, None) == E.BAD_ARG
