@@ -96,7 +96,12 @@ class PagedDecoder:
                 return i
         raise E.MCPMError(E.BAD_ARG, "no free sequence")
 
+    def _names_one(self, seq: int) -> bool:
+        return 0 <= operator.index(seq) < self.max_seqs
+
     def close(self, seq: int) -> None:
+        if not self._names_one(seq):
+            raise E.MCPMError(E.BAD_ARG, f"sequence {seq}")
         self._give_back(seq)
         self.opened[seq] = False
         self.length[seq] = 0
@@ -141,8 +146,10 @@ class PagedDecoder:
         evicts.  Pages are counted in the step's own order: an eviction takes its fresh ones before it frees the old."""
         evicted, free = [], len(self.free)
         for s, token in tokens.items():
-            if not self.opened[s] or not 0 <= operator.index(token) < self.n_vocab:
-                raise E.MCPMError(E.BAD_TOKEN if self.opened[s] else E.BAD_ARG, f"sequence {s}")
+            if not self._names_one(s) or not self.opened[s]:
+                raise E.MCPMError(E.BAD_ARG, f"sequence {s}")
+            if not 0 <= operator.index(token) < self.n_vocab:
+                raise E.MCPMError(E.BAD_TOKEN, f"sequence {s}")
             length, fresh = int(self.length[s]), 0
             if self.keep and length >= self.keep + self.slack:
                 evicted.append(s)

@@ -125,3 +125,20 @@ def test_limits_are_the_operators_own():
     for more in (dict(hist=256, penalties=256, hist_max=E.MAX_HIST + 1), dict(bias_token=256, bias=256, bias_max=E.MAX_BIAS + 1)):
         p = E.mcpm_logits_params(n_seq=1, n_vocab=100, logits=256, out=512, **more)
         assert lib.mcpm_logits_process(p, None) == E.BAD_ARG
+
+
+def test_sequence_numbers_are_not_indexes_from_the_end():
+    """-1 names no sequence: with 1 it would feed two tokens to one slot of the last."""
+    from mcpm import engine as E
+    d = decoder(6, 2, [3, 5])
+    for tokens in ({-1: 1}, {1: 1, -1: 2}, {0: 1, 2: 1}):
+        refused(d, E.BAD_ARG, tokens)
+    refused(d, TypeError, {0.5: 1})
+    before = state(d)
+    for s in (-1, 2):
+        with pytest.raises(E.MCPMError) as e:
+            d.close(s)
+        assert e.value.status == E.BAD_ARG and state(d) == before
+    d.close(1)
+    d.close(1)   # an unused one: nothing to do
+    assert len(d.free) == 5
