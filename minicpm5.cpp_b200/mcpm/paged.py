@@ -44,8 +44,9 @@ class PagedDecoder:
     def __init__(self, path: str, n_pages: int, page_size: int = 16, max_seqs: int = 1, max_positions: int = 1024,
                  kv_type: int = E.KV_F32, keep: int = 0, slack: int = 16, sink: int = 4, recent: int = 16,
                  rope_len: int = 16384):
-        if keep and (sink + recent > keep or keep + slack > max_positions):
-            raise ValueError("sink + recent <= keep, keep + slack <= max_positions")
+        max_pages = -(-max_positions // page_size)
+        if keep and (min(keep, slack, sink, recent) < 0 or sink + recent > keep or keep + slack > max_positions or keep >= max_pages * page_size):
+            raise ValueError("0 <= sink + recent <= keep, 0 <= slack, keep + slack <= max_positions, room for a position beyond keep")
         _, tensors, _ = gguf.read_header(path)
         self.tensors = {t.name: t for t in tensors}
         self.n_layer = sum(name.endswith("attn_q.weight") for name in self.tensors)
@@ -59,7 +60,6 @@ class PagedDecoder:
         self.weights = {name: torch.from_numpy(np.array(self.file[t.offset:t.offset + t.nbytes])).cuda()
                         for name, t in self.tensors.items() if name != "token_embd.weight"}
         self.page_size, self.max_seqs, self.keep, self.slack, self.sink, self.recent = page_size, max_seqs, keep, slack, sink, recent
-        max_pages = -(-max_positions // page_size)
         self.max_positions = max_pages * page_size
         self.cfg = E.paged_config(kv_type, spec.N_HEAD, spec.N_HEAD_KV, spec.HEAD_DIM, page_size, n_pages, max_seqs, max_pages)
         dtype = {E.KV_F32: torch.float32, E.KV_F16: torch.float16, E.KV_BF16: torch.bfloat16}[kv_type]

@@ -142,3 +142,14 @@ def test_sequence_numbers_are_not_indexes_from_the_end():
     d.close(1)
     d.close(1)   # an unused one: nothing to do
     assert len(d.free) == 5
+
+
+@pytest.mark.parametrize("budget", [dict(slack=-1), dict(slack=-32), dict(sink=-1), dict(recent=-1, sink=20), dict(keep=-1), dict(keep=64, slack=0),
+                                    dict(slack=33), dict(sink=30, recent=3)])
+def test_budgets_that_cannot_be_kept(budget):
+    """With a negative slack a sequence was cut to `keep` positions while it still had fewer, and attended to slots that
+    nothing had been written to.  Refused before the file is opened."""
+    from mcpm import paged
+    with pytest.raises(ValueError) as e:
+        paged.PagedDecoder("no such file", n_pages=8, max_positions=64, **{**dict(keep=32, sink=2, recent=8), **budget})
+    assert "keep" in str(e.value)
