@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import argparse
 import operator
+import os
 import time
 from typing import Dict, List, Optional, Tuple
 
@@ -37,6 +38,31 @@ def dequantize_q4_k(raw: np.ndarray) -> np.ndarray:
     return ((d * scale)[:, :, None] * vals - (dmin * low)[:, :, None]).reshape(-1, 256)
 
 
+def model_tensors(path: str) -> Tuple[Dict[str, spec.TensorInfo], int]:
+    """The tensors that a decoder reads, by name, and the number of layers.  Their shapes size every buffer of the
+    kernels, so a file of another shape, or one that ends early, is refused here."""
+    size = os.path.getsize(path)
+    there = {t.name: t for t in gguf.read_header(path)[1]}
+    n_layer = 0
+    while f"blk.{n_layer}.attn_q.weight" in there:
+        n_layer += 1
+    emb = there.get("token_embd.weight")
+    vocab = emb.dims[1] if emb is not None and len(emb.dims) == 2 else 0
+    want = {"token_embd.weight": (spec.N_EMBD, vocab), "output.weight": (spec.N_EMBD, vocab), "output_norm.weight": (spec.N_EMBD,)}
+    for i in range(n_layer):
+        want.update({f"blk.{i}.{base}.weight": spec.layer_dims(base) for base in spec.LAYER_TENSORS})
+    for name, dims in want.items():
+        t = there.get(name)
+        if not n_layer or not vocab or t is None or t.dims != dims:
+            raise E.MCPMError(E.BAD_FILE, f"{name}: {'absent' if t is None else t.dims}, expected {dims}")
+        types = (spec.GGML_F32,) if len(dims) == 1 else (spec.GGML_Q4_K,) if t is emb else (spec.GGML_Q4_K, spec.GGML_Q6_K)
+        if t.ggml_type not in types:
+            raise E.MCPMError(E.UNSUPPORTED_TYPE, f"{name}: the paged decoder reads Q4_K_M files")
+        if t.offset + t.nbytes > size:
+            raise E.MCPMError(E.BAD_FILE, f"{name}: beyond the end of the file")
+    return {name: there[name] for name in want}, n_layer
+
+
 class PagedDecoder:
     """keep: positions that a sequence has after an eviction, which comes when it reaches keep + slack of them
     (0: never evicted); sink and recent of them are always the first and the last ones."""
@@ -47,16 +73,12 @@ class PagedDecoder:
         max_pages = -(-max_positions // page_size)
         if keep and (min(keep, slack, sink, recent) < 0 or sink + recent > keep or keep + slack > max_positions or keep >= max_pages * page_size):
             raise ValueError("0 <= sink + recent <= keep, 0 <= slack, keep + slack <= max_positions, room for a position beyond keep")
-        _, tensors, _ = gguf.read_header(path)
-        self.tensors = {t.name: t for t in tensors}
-        self.n_layer = sum(name.endswith("attn_q.weight") for name in self.tensors)
+        self.tensors, self.n_layer = model_tensors(path)
         emb = self.tensors["token_embd.weight"]
-        if emb.ggml_type != E.Q4_K:
-            raise E.MCPMError(E.UNSUPPORTED_TYPE, "token_embd: the paged decoder reads Q4_K_M files")
         self.n_vocab = emb.dims[1]
         self.file = np.memmap(path, np.uint8, "r")
         self.embeddings = self.file[emb.offset:emb.offset + emb.nbytes].reshape(self.n_vocab, -1, 144)
-        # everything but the embeddings, as it lies in the file; tensors are 32-byte aligned there
+        # everything but the embeddings, as it lies in the file
         self.weights = {name: torch.from_numpy(np.array(self.file[t.offset:t.offset + t.nbytes])).cuda()
                         for name, t in self.tensors.items() if name != "token_embd.weight"}
         self.page_size, self.max_seqs, self.keep, self.slack, self.sink, self.recent = page_size, max_seqs, keep, slack, sink, recent

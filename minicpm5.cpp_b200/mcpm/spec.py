@@ -83,7 +83,7 @@ def q4km_uses_q6k(layer: int, n_layer: int = N_LAYER) -> bool:
     return layer < eighth or layer >= 7 * n_layer // 8 or (layer - eighth) % 3 == 2
 
 
-def _dims(base: str) -> Tuple[int, ...]:
+def layer_dims(base: str) -> Tuple[int, ...]:
     return {
         "attn_q": (N_EMBD, N_EMBD), "attn_k": (N_EMBD, KV_DIM), "attn_v": (N_EMBD, KV_DIM),
         "attn_output": (N_EMBD, N_EMBD), "ffn_gate": (N_EMBD, N_FF), "ffn_up": (N_EMBD, N_FF),
@@ -115,7 +115,7 @@ def tensor_list(variant: str = "q4_k_m") -> List[TensorInfo]:
                 t = GGML_Q6_K
             else:
                 t = GGML_Q4_K
-            out.append(TensorInfo(f"blk.{layer}.{base}.weight", t, _dims(base)))
+            out.append(TensorInfo(f"blk.{layer}.{base}.weight", t, layer_dims(base)))
     return out
 
 

@@ -153,3 +153,45 @@ def test_budgets_that_cannot_be_kept(budget):
     with pytest.raises(ValueError) as e:
         paged.PagedDecoder("no such file", n_pages=8, max_positions=64, **{**dict(keep=32, sink=2, recent=8), **budget})
     assert "keep" in str(e.value)
+
+
+def write_header(path, change=lambda t: t, short=0):
+    """A model file without weights: the header, and a hole of the data section's size less `short` bytes."""
+    from mcpm import spec, synth
+    tensors = [t for t in map(change, spec.tensor_list("q4_k_m")) if t is not None and (not t.name.startswith("blk.") or t.name.startswith("blk.0."))]
+    tensors = spec.layout(tensors, spec.Q4KM_DATA_START)
+    with open(path, "wb") as f:
+        f.write(synth._header(tensors, spec.Q4KM_DATA_START, "q4_k_m"))
+        f.truncate(tensors[-1].offset + tensors[-1].nbytes - short)
+    return str(path)
+
+
+def test_model_file(tmp_path):
+    from mcpm import paged, spec
+    tensors, n_layer = paged.model_tensors(write_header(tmp_path / "m.gguf"))
+    assert n_layer == 1 and len(tensors) == 3 + len(spec.LAYER_TENSORS)
+    assert tensors["blk.0.ffn_down.weight"].dims == (spec.N_FF, spec.N_EMBD)
+
+
+@pytest.mark.parametrize("name,dims,kind,status", [
+    ("blk.0.ffn_gate.weight", (2048, 8192), 12, "BAD_FILE"), ("blk.0.ffn_down.weight", (8192, 2048), 14, "BAD_FILE"),
+    ("blk.0.attn_k.weight", (2048, 2048), 12, "BAD_FILE"), ("output.weight", (2048, 131072), 14, "BAD_FILE"),
+    ("blk.0.attn_norm.weight", (1024,), 0, "BAD_FILE"), ("token_embd.weight", (4096, 130560), 12, "BAD_FILE"),
+    ("blk.0.attn_v.weight", None, 12, "BAD_FILE"), ("blk.0.attn_q.weight", None, 12, "BAD_FILE"), ("output_norm.weight", None, 0, "BAD_FILE"),
+    ("token_embd.weight", (2048, 130560), 14, "UNSUPPORTED_TYPE"), ("blk.0.attn_q.weight", (2048, 2048), 8, "UNSUPPORTED_TYPE"),
+    ("blk.0.ffn_norm.weight", (2048,), 1, "UNSUPPORTED_TYPE")])
+def test_models_of_another_shape_are_refused(tmp_path, name, dims, kind, status):
+    """Wider layers would have written beyond the decoder's buffers.  Refused before anything is uploaded."""
+    from mcpm import engine as E, paged, spec
+    path = write_header(tmp_path / "m.gguf", lambda t: t if t.name != name else dims and spec.TensorInfo(name, kind, dims))
+    with pytest.raises(E.MCPMError) as e:
+        paged.PagedDecoder(path, n_pages=4)
+    assert e.value.status == getattr(E, status)
+
+
+def test_a_truncated_model_is_refused(tmp_path):
+    """The last tensor's missing bytes would have been read beyond its copy on the device."""
+    from mcpm import engine as E, paged
+    with pytest.raises(E.MCPMError) as e:
+        paged.PagedDecoder(write_header(tmp_path / "m.gguf", short=1), n_pages=4)
+    assert e.value.status == E.BAD_FILE
