@@ -65,7 +65,8 @@ def model_tensors(path: str) -> Tuple[Dict[str, spec.TensorInfo], int]:
 
 class PagedDecoder:
     """keep: positions that a sequence has after an eviction, which comes when it reaches keep + slack of them
-    (0: never evicted); sink and recent of them are always the first and the last ones."""
+    (0: never evicted); sink and recent of them are always the first and the last ones.  rope_len: positions that the
+    RoPE table has at first; it doubles when a sequence comes to its end (512 bytes a position)."""
 
     def __init__(self, path: str, n_pages: int, page_size: int = 16, max_seqs: int = 1, max_positions: int = 1024,
                  kv_type: int = E.KV_F32, keep: int = 0, slack: int = 16, sink: int = 4, recent: int = 16,
@@ -90,7 +91,7 @@ class PagedDecoder:
         self.mass = torch.zeros((self.n_layer, n_pages, spec.N_HEAD_KV, page_size), device="cuda")
         self.pools = [E.paged_pool(self.k[i].data_ptr(), self.v[i].data_ptr(), self.mass[i].data_ptr()) for i in range(self.n_layer)]
         self.workspace = torch.zeros(E.paged_workspace_bytes(self.cfg), dtype=torch.uint8, device="cuda")
-        self.rope = torch.from_numpy(E.rope_table(rope_len, spec.HEAD_DIM, spec.ROPE_BASE)).cuda()
+        self.rope = self._rope_table(rope_len)
         # host state: a row per open sequence
         self.free: List[int] = list(range(n_pages))[::-1]
         self.table = np.full((max_seqs, max_pages), -1, np.int32)
@@ -159,6 +160,15 @@ class PagedDecoder:
     def _stream() -> int:
         return torch.cuda.current_stream().cuda_stream
 
+    @staticmethod
+    def _rope_table(n: int) -> torch.Tensor:
+        return torch.from_numpy(E.rope_table(n, spec.HEAD_DIM, spec.ROPE_BASE)).cuda()
+
+    def _reach(self, position: int) -> None:
+        """Extends the RoPE table to a position: positions count on where the cache is bounded."""
+        if position >= self.rope.shape[0]:
+            self.rope = self._rope_table(max(2 * self.rope.shape[0], position + 1))
+
     # ---------------------------------------------------------------- one step
     def _needs_page(self, seq: int, length: int) -> bool:
         return length % self.page_size == 0 and self.table[seq, length // self.page_size] < 0
@@ -176,7 +186,7 @@ class PagedDecoder:
             if self.keep and length >= self.keep + self.slack:
                 evicted.append(s)
                 fresh, length = -(-self.keep // self.page_size), self.keep
-            if length >= self.max_positions or self.position[s] >= self.rope.shape[0]:
+            if length >= self.max_positions:
                 raise E.MCPMError(E.CTX_OVERFLOW, f"sequence {s}")
             more = length % self.page_size == 0 if fresh else self._needs_page(s, length)
             held = int((self.table[s] >= 0).sum()) if fresh else 0
@@ -201,7 +211,7 @@ class PagedDecoder:
         if (repetition, frequency, presence) != (1.0, 0.0, 0.0):
             if not repetition > 0:
                 raise E.MCPMError(E.BAD_ARG, "repetition > 0")
-            rows = [self.history[s] + [t] for s, t in tokens.items()]
+            rows = [self.history[s][1 - E.MAX_HIST:] + [t] for s, t in tokens.items()]
             hist = np.full((n, max(map(len, rows))), -1, np.int32)
             for r, row in enumerate(rows):
                 hist[r, :len(row)] = row
@@ -227,11 +237,13 @@ class PagedDecoder:
     def step(self, tokens: Dict[int, int], repetition: float = 1.0, frequency: float = 0.0, presence: float = 0.0,
              bias: Optional[Dict[int, float]] = None, allow: Optional[np.ndarray] = None) -> Dict[int, int]:
         """Feeds one token to each given sequence and returns their greedy next tokens (-1: the grammar allows none).
-        Penalties count the tokens fed so far; allow: bool [n_vocab] or [len(tokens)][n_vocab]."""
+        Penalties count the tokens fed so far (the last 1048575 of them; the lists are laid out and copied anew in each
+        step that has penalties); allow: bool [n_vocab] or [len(tokens)][n_vocab]."""
         seqs = list(tokens)
         n = len(seqs)
         evicted = self._check(tokens)
         held, more = self._options(tokens, repetition, frequency, presence, bias, allow)   # held: the lists' memory
+        self._reach(max(int(self.position[s]) for s in seqs))
         self._admit(seqs, evicted)
         st, ws = self._stream(), (self.workspace.data_ptr(), self.workspace.numel())
         table, slot = self._dev(self.table[seqs]), self._dev(self.length[seqs])

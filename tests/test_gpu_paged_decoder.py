@@ -242,3 +242,19 @@ def test_a_refused_option_can_be_corrected(cuda, parity):
 
     a, b = run(False), run(True)
     assert a[0] == b[0] and np.array_equal(a[1], b[1])
+
+
+@pytest.mark.gpu
+def test_a_conversation_outlives_its_rope_table(cuda, parity):
+    """Positions beyond the first table rotate as with one that was long enough."""
+    from mcpm import paged, synth
+    _, _, path = parity
+    ids = [int(t) for t in synth.prompt_ids(60, seed=12)]
+
+    def run(rope_len):
+        d = paged.PagedDecoder(path, n_pages=8, max_positions=64, keep=20, slack=16, sink=2, recent=8, rope_len=rope_len)
+        s = d.open()
+        return [d.step({s: t})[s] for t in ids], d.logits[0].cpu().numpy(), d.k.cpu().numpy()
+
+    a, b = run(4), run(64)
+    assert a[0] == b[0] and np.array_equal(a[1], b[1]) and np.array_equal(a[2], b[2])

@@ -195,3 +195,29 @@ def test_a_truncated_model_is_refused(tmp_path):
     with pytest.raises(E.MCPMError) as e:
         paged.PagedDecoder(write_header(tmp_path / "m.gguf", short=1), n_pages=4)
     assert e.value.status == E.BAD_FILE
+
+
+def test_positions_count_beyond_the_first_rope_table():
+    """A sequence whose cache is bounded does not end where the table of rotations did."""
+    d = decoder(6, 2, [10, 20], keep=32, rope_len=30)
+    d.position[:] = [10, 30]
+    assert d._check({0: 1, 1: 1}) == []
+    made = []
+    d._rope_table = lambda n: made.append(n) or np.zeros((n, 64, 2), np.float32)
+    for p in (10, 29, 30, 59, 60, 500):
+        d._reach(p)
+        assert d.rope.shape[0] > p
+    assert made == [60, 120, 501]
+
+
+def test_histories_beyond_the_operators_limit():
+    """Penalties count the last tokens that the operator takes; a long conversation is not refused."""
+    from mcpm import engine as E
+    d = decoder(6, 2, [16, 16])
+    d._dev = lambda a, dtype=np.int32: torch.from_numpy(np.ascontiguousarray(a, dtype=dtype))
+    d.history = [[3] * 5 + [4] * (E.MAX_HIST - 1), [5, 6]]
+    held, more = d._options({0: 9, 1: 8}, 1.1, 0.0, 0.0, None, None)
+    hist = held[0].numpy()
+    assert hist.shape == (2, E.MAX_HIST) and more["hist_stride"] == E.MAX_HIST
+    assert (hist[0, :-1] == 4).all() and hist[0, -1] == 9
+    assert hist[1, :3].tolist() == [5, 6, 8] and (hist[1, 3:] == -1).all()
