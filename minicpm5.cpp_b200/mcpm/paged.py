@@ -66,7 +66,11 @@ def model_tensors(path: str) -> Tuple[Dict[str, spec.TensorInfo], int]:
 class PagedDecoder:
     """keep: positions that a sequence has after an eviction, which comes when it reaches keep + slack of them
     (0: never evicted); sink and recent of them are always the first and the last ones.  rope_len: positions that the
-    RoPE table has at first; it doubles when a sequence comes to its end (512 bytes a position)."""
+    RoPE table has at first; it doubles when a sequence comes to its end (512 bytes a position).
+
+    An eviction copies to ceil(keep / page_size) free pages before it frees the old ones, one sequence after the other:
+    with max_seqs * ceil((keep + max(slack, 1)) / page_size) + ceil(keep / page_size) pages the pool never runs out.  A
+    step that would need more than are free is refused as a whole (OOM)."""
 
     def __init__(self, path: str, n_pages: int, page_size: int = 16, max_seqs: int = 1, max_positions: int = 1024,
                  kv_type: int = E.KV_F32, keep: int = 0, slack: int = 16, sink: int = 4, recent: int = 16,

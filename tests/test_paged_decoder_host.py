@@ -221,3 +221,18 @@ def test_histories_beyond_the_operators_limit():
     assert hist.shape == (2, E.MAX_HIST) and more["hist_stride"] == E.MAX_HIST
     assert (hist[0, :-1] == 4).all() and hist[0, -1] == 9
     assert hist[1, :3].tolist() == [5, 6, 8] and (hist[1, 3:] == -1).all()
+
+
+@pytest.mark.parametrize("page_size,keep,slack", [(16, 32, 16), (16, 20, 0), (16, 33, 5), (7, 40, 3), (1, 20, 7)])
+def test_the_stated_pages_are_enough(page_size, keep, slack):
+    """Sequences at their budgets in one pool, stepped together in any order, never run out of pages."""
+    n = 3 * -(-(keep + max(slack, 1)) // page_size) + -(-keep // page_size)
+    d = decoder(n, 3, [0, 0, 0], page_size=page_size, max_positions=-(-(keep + slack + 1) // page_size) * page_size, keep=keep, slack=slack,
+                sink=2, recent=8)
+    rng = np.random.default_rng(page_size)
+    for _ in range(400):
+        seqs = [int(s) for s in rng.permutation(3)[:rng.integers(1, 4)]]
+        d._admit(seqs, d._check({s: 1 for s in seqs}))
+        d.length[seqs] += 1
+        assert len(d.free) + int((d.table >= 0).sum()) == n
+    assert d.evictions and all_pages(d, n)
