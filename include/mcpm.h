@@ -356,7 +356,9 @@ typedef struct {
  * q and k by interleaved pairs (2i, 2i+1) as mcpm_rope_kv_append does, rounds k and v to the cache
  * type (nearest, ties to even) into slot tok_slot of sequence tok_seq, and zeroes the mass of those
  * positions.  No two tokens of a call may name the same slot.  Rows 16-byte aligned.
- * table: [n_seq][max_pages]; tok_seq outside [0, n_seq) is padding. */
+ * table: [n_seq][max_pages].  A token with a negative slot or a tok_seq outside [0, n_seq) is padding:
+ * nothing is written for it, its row of q_out included.  A slot beyond the table or in an absent page
+ * drops the token's K and V; its query is rotated all the same. */
 mcpm_status mcpm_paged_append(const mcpm_paged_config* cfg, const mcpm_paged_pool* pool, const int* table, int n_seq,
                               const mcpm_paged_tokens* tokens, void* stream);
 /* GQA attention of one query per sequence over its pages (execute_attention, ops.cpp:537-628, on a

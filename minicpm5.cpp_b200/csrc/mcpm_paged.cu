@@ -36,12 +36,13 @@ __global__ void __launch_bounds__(32 * AP_WARPS) k_paged_append(const PagedGeom 
     const size_t i = blockIdx.x;
     const int x = threadIdx.x % LANES, first = threadIdx.x / LANES, nq = a.t.q ? g.n_head : 0, nk = g.n_head_kv, rows = nq + 2 * nk;
     const int tok_slot = a.t.tok_slot[i], seq = a.t.tok_seq ? a.t.tok_seq[i] : static_cast<int>(i);
+    // Slots of the token's sequence, 0: padding.  The stores alone look at it, so the loads do not wait for it.
+    const unsigned slots = tok_slot >= 0 && seq >= 0 && seq < a.n_seq ? static_cast<unsigned>(g.max_pages * g.page_size) : 0u;
     const int pos = a.t.tok_pos ? a.t.tok_pos[i] : tok_slot;
     const float4 cs = a.t.rope ? reinterpret_cast<const float4*>(a.t.rope)[static_cast<size_t>(min(max(pos, 0), a.t.rope_len - 1)) * LANES + x]
                                : make_float4(1.0f, 0.0f, 1.0f, 0.0f);
     int page = -1, slot = 0;
-    const bool held = seq >= 0 && seq < a.n_seq && tok_slot >= 0 && tok_slot < g.max_pages * g.page_size &&
-                      g.locate(a.table + static_cast<size_t>(seq) * g.max_pages, tok_slot, page, slot);
+    const bool held = static_cast<unsigned>(tok_slot) < slots && g.locate(a.table + static_cast<size_t>(seq) * g.max_pages, tok_slot, page, slot);
     for (int r0 = first; r0 < rows; r0 += AT_ONCE * AP_HELD) {
         float4 v[AP_HELD];
 #pragma unroll
@@ -61,7 +62,7 @@ __global__ void __launch_bounds__(32 * AP_WARPS) k_paged_append(const PagedGeom 
                 y = make_float4(__fmaf_rn(cs.x, y.x, -__fmul_rn(cs.y, y.y)), __fmaf_rn(cs.y, y.x, __fmul_rn(cs.x, y.y)),
                                 __fmaf_rn(cs.z, y.z, -__fmul_rn(cs.w, y.w)), __fmaf_rn(cs.w, y.z, __fmul_rn(cs.z, y.w)));
             if (r < nq) {
-                reinterpret_cast<float4*>(a.t.q_out + (i * g.n_head + r) * D)[x] = y;
+                if (slots) reinterpret_cast<float4*>(a.t.q_out + (i * g.n_head + r) * D)[x] = y;
             } else if (held) {
                 const bool is_v = r >= nq + nk;
                 const int head = r - nq - (is_v ? nk : 0);

@@ -375,6 +375,40 @@ def test_append_padding_and_defaults(cuda):
     assert cuda.equal(before[0], c.k) and cuda.equal(before[1], c.v)
 
 
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("seqs", [False, True])
+def test_append_leaves_the_queries_of_padding_alone(cuda, in_place, seqs):
+    """A padding token's row of q_out keeps what it held, with and without tok_pos; a token whose page is absent has its
+    query rotated."""
+    c = Cache(cuda, "f16", 4, 2, 64, 16, [64] * 6, seed=40)
+    c.table[3, 0] = -1
+    q, k, v = cuda.randn(6, 256, device="cuda"), cuda.randn(6, 128, device="cuda"), cuda.randn(6, 128, device="cuda")
+    slot = np.array([5, -1, 9, 3, -2 ** 31, 64], np.int32)
+    seq = np.array([0, 1, 6 if seqs else 2, 3, 4, 5], np.int32)
+    q0, pad = q.clone(), np.array([1, 2, 4] if seqs else [1, 4])
+    out = q if in_place else cuda.full_like(q, 7.0)
+    rope = c.dev(c.E.rope_table(100, 64))
+    d = [c.dev(x) for x in (slot, seq, c.table)]
+    k1, v1 = c.k.clone(), c.v.clone()
+    c.E.paged_append(c.cfg, c.pool, d[2].data_ptr(), 6, d[0].data_ptr(), k.data_ptr(), v.data_ptr(), tok_seq=d[1].data_ptr() if seqs else 0,
+                     q=q.data_ptr(), q_out=out.data_ptr(), rope=rope.data_ptr(), rope_len=100)
+    cuda.cuda.synchronize()
+    real = np.setdiff1d(np.arange(6), pad)
+    assert cuda.equal(out[c.dev(pad)], q0[c.dev(pad)] if in_place else cuda.full_like(q0[:pad.size], 7.0))
+    cs = c.dev(c.E.rope_table(100, 64)[slot[real]]).double()[:, None]
+    a, b = q0[c.dev(real)].double().view(-1, 4, 32, 2).unbind(-1)
+    want = cuda.stack([cs[..., 0] * a - cs[..., 1] * b, cs[..., 1] * a + cs[..., 0] * b], -1)
+    size = cuda.stack([(cs[..., 0] * a).abs() + (cs[..., 1] * b).abs(), (cs[..., 1] * a).abs() + (cs[..., 0] * b).abs()], -1)
+    got = out[c.dev(real)].double().view(-1, 4, 32, 2)
+    assert bool(((got - want).abs() <= 2 * 2.0 ** -24 * size).all())   # two roundings
+    for i in real:
+        if slot[i] < 64 and c.table[i, slot[i] // 16] >= 0:
+            p = int(c.table[i, slot[i] // 16])
+            k1[p, slot[i] % 16], v1[p, slot[i] % 16] = c.k[p, slot[i] % 16], c.v[p, slot[i] % 16]
+            assert cuda.equal(c.v[p, slot[i] % 16], v[i].view(2, 64).half())
+    assert cuda.equal(k1, c.k) and cuda.equal(v1, c.v)
+
+
 # ------------------------------------------------------------------ eviction
 def expected_kept(mass, j, n, keep, sink, recent):
     m = mass.astype(np.float64).copy()
