@@ -366,7 +366,10 @@ mcpm_status mcpm_paged_append(const mcpm_paged_config* cfg, const mcpm_paged_poo
  * sequence that sees none gets zeros.  q and out: rows of n_head * head_dim floats, q_stride floats
  * between the rows of q (0: packed).  scale 0: 1/sqrt(head_dim).  With pool->mass, each visible
  * position's mass grows by the sum of its weights over the g query heads of its KV head; the
- * sequences of such a call share no pages.  Results do not depend on how the work was split over
+ * sequences of such a call share no pages.  Scores, and sums of exp(score - largest score) |V|, are held
+ * in fp32: K and V may be as large as their type allows where these stay below 2e38.  K and V of the
+ * visible positions are finite; where one is not, outputs and masses of its KV head in that sequence may be
+ * NaN, and nothing else is touched.  Results do not depend on how the work was split over
  * the GPU in other calls: equal inputs give equal bits. */
 mcpm_status mcpm_paged_attention(const mcpm_paged_config* cfg, const mcpm_paged_pool* pool, const int* table,
                                  const int* seq_len, int n_seq, const float* q, int64_t q_stride, float* out,

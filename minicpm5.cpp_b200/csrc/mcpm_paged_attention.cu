@@ -41,11 +41,18 @@ constexpr int FAN = 16, FAN_BITS = 4, LEVELS = 3;   // records joined at a time,
 // with its arrival and join than as work.
 constexpr int WHOLE = 2, LEAD = 1;   // LEAD 1, 2, 3: 30.6, 31.6, 32.8 us at 200 sequences of 20 to 900 fp16 positions
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr float P_SCALE = 1024.0f;  // weights are multiplied by this before they are split: fp16 parts of small
-                                    // weights stay normal; undone in the output
 
 template <typename T>
 constexpr int parts() { return sizeof(T) == 4 || __is_same(T, __half) ? 2 : 3; }
+// Powers of two that keep parts and products in range.  fp16 parts have five bits of exponent: weights are multiplied
+// by 1024 and q brought to [2^7, 2^8), so that the parts of small ones stay normal, and no product of values up to
+// 65504 comes near the end of fp32.  The other parts have fp32's eight bits: weights stay as they are, and q is brought
+// to [2^-8, 2^-7), where 128 products with finite values cannot exceed the largest of them.  Undone in the output and
+// in the factor of the scores.
+template <typename T>
+constexpr float p_scale() { return __is_same(T, __half) ? 1024.0f : 1.0f; }
+template <typename T>
+constexpr int q_exponent() { return __is_same(T, __half) ? 7 : -8; }
 
 template <typename T, int D, int NT>
 struct Tile {
@@ -409,7 +416,7 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
                         x = make_float4(fmaf(r[j].x, e, x.x), fmaf(r[j].y, e, x.y), fmaf(r[j].z, e, x.z), fmaf(r[j].w, e, x.w));
                     }
                 }
-                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum, f = done ? inv * (1.0f / P_SCALE) : 1.0f;
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum, f = done ? inv * (1.0f / p_scale<T>()) : 1.0f;
                 const float4 y = make_float4(x.x * f, x.y * f, x.z * f, x.w * f);
                 if (done) {
                     if (mine) reinterpret_cast<float4*>(out)[i] = y;
@@ -432,8 +439,7 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
 
     int before_slot, k_slot, v_slot = L::SLOTS - 1;   // slots of the last tile's V and of this tile's K and V
     for (int k = 0; seg0 < end;) {
-        // ---- q in fragment order, normalised per head to [2^7, 2^8) so that 16-bit parts neither overflow
-        // nor vanish
+        // ---- q in fragment order, normalised per head
 #pragma unroll
         for (int qi = 0; qi < NT; ++qi) {
             const int h = warp + WARPS * qi;
@@ -441,7 +447,7 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
             float top = 0.0f;
             for (int i = 0; i < D / 32; ++i) top = fmaxf(top, fabsf(x[i]));
             for (int o = 16; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const int e = min(max(7 - (static_cast<int>(__float_as_uint(top) >> 23) - 127), -120), 120);
+            const int e = min(max(q_exponent<T>() - (static_cast<int>(__float_as_uint(top) >> 23) - 127), -120), 120);
             const float up = pow2(e);
 #pragma unroll
             for (int i = 0; i < D / 32; ++i) {
@@ -459,7 +465,7 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
                     for (int k = 0; k < parts<T>(); ++k) p[4 * k] = take_part<T>(v);
                 }
             }
-            if (lane == 0) s_qf[h] = a.scale * LOG2E * pow2(-e);
+            if (lane == 0) s_qf[h] = a.scale * pow2(-e) * LOG2E;   // in this order: a scale for large K may be subnormal
         }
         __syncthreads();
         float qf[NT][2];
@@ -578,8 +584,8 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
                     p[nt][i] = where0 >= 0 ? fast_exp2(__fmaf_rn(s[nt][i], qf[nt][i], -ref)) : 0.0f;
                     p[nt][2 + i] = where1 >= 0 ? fast_exp2(__fmaf_rn(s[nt][2 + i], qf[nt][i], -ref)) : 0.0f;
                     l[nt][i] += p[nt][i] + p[nt][2 + i];
-                    p[nt][i] *= P_SCALE;
-                    p[nt][2 + i] *= P_SCALE;
+                    p[nt][i] *= p_scale<T>();
+                    p[nt][2 + i] *= p_scale<T>();
                 }
             cp_async_wait_group<L::SLOTS - 2>();
             __syncwarp();   // V is there, and all lanes are done with K
@@ -715,7 +721,7 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
             }
             if (whole) {
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                s_inv[tid] = inv * (1.0f / P_SCALE);
+                s_inv[tid] = inv * (1.0f / p_scale<T>());
                 if (MASS) a.stats[static_cast<size_t>(at_seq) * g.n_head + at_kv * group + tid] = make_float2(top, inv);
             } else {
                 s_inv[tid] = 1.0f;

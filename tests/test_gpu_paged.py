@@ -207,6 +207,46 @@ def test_attention_query_magnitudes(cuda, kv, size):
     assert np.all(np.abs(got - want) <= tol), np.max(np.abs(got - want) / tol)
 
 
+@pytest.mark.parametrize("kv", ["f32", "bf16"])
+@pytest.mark.parametrize("k_size,v_size", [(1e37, 1.0), (1.0, 1e36), (3e37, 3e36), (1e-20, 1e-15), (1e37, 1e-15)])
+def test_attention_cache_magnitudes(cuda, kv, k_size, v_size):
+    """K and V up to the ends of their types' range, with queries and a scale that make the scores ordinary.  At most
+    7 x 3e36 x 12: sums over the 12 positions stay in range."""
+    c = Cache(cuda, kv, 16, 2, 128, 16, [12, 9], seed=41, mass=False)
+    c.k *= k_size
+    c.v *= v_size
+    assert bool(cuda.isfinite(c.k).all() & cuda.isfinite(c.v).all())
+    for q_size in (1e-12, 1.0):
+        q = q_size * cuda.randn(2, 2048, device="cuda")
+        scale = float(np.float32(0.1 / q_size / k_size))
+        want, tol, _, _ = expected_attention(c, q, scale)
+        got = c.attend(q, scale=scale).double().cpu().numpy()
+        assert np.all(np.abs(got - want) <= tol), np.max(np.abs(got - want) / tol)
+
+
+@pytest.mark.parametrize("kv", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")])
+def test_attention_values_that_are_not_finite_stay_in_their_head(cuda, kv, bad):
+    """One infinite or NaN element of K or of V at a visible position: other KV heads, other sequences and, for V, other
+    dims keep their bits; masses of the other KV head too."""
+    def fresh():
+        return Cache(cuda, kv, 16, 2, 128, 16, [300, 77], seed=43)
+    q = cuda.randn(2, 2048, device="cuda")
+    c = fresh()
+    want, mass = c.attend(q).view(2, 2, 8, 128), c.mass.clone()
+    _, p, s = c.places(0)
+    for pool in ("k", "v"):
+        d = fresh()
+        getattr(d, pool)[int(p[150]), int(s[150]), 1, 5] = bad
+        got = d.attend(q).view(2, 2, 8, 128)
+        assert cuda.equal(got[1], want[1]) and cuda.equal(got[0, 0], want[0, 0])
+        assert cuda.equal(d.mass[:, 0], mass[:, 0])
+        if pool == "v":
+            other = cuda.arange(128, device="cuda") != 5
+            assert cuda.equal(got[0, 1][:, other], want[0, 1][:, other]) and cuda.equal(d.mass, mass)
+            assert not bool(cuda.isfinite(got[0, 1, :, 5]).any())
+
+
 def test_attention_same_bits_and_no_trace_of_other_calls(cuda):
     """Equal inputs give equal bits, whatever ran on the workspace in between, on another stream too."""
     c = Cache(cuda, "f16", 16, 2, 128, 16, [3000, 5, 1200, 0, 64], seed=11, mass=False)
