@@ -581,8 +581,13 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const float ref = m[nt][i] == -INFINITY ? 0.0f : m[nt][i];
-                    p[nt][i] = where0 >= 0 ? fast_exp2(__fmaf_rn(s[nt][i], qf[nt][i], -ref)) : 0.0f;
-                    p[nt][2 + i] = where1 >= 0 ? fast_exp2(__fmaf_rn(s[nt][2 + i], qf[nt][i], -ref)) : 0.0f;
+                    // s qf - ref without the product's rounding (at most 2^-17 here), which a pair's weights then share as
+                    // a factor.  With it beyond 128: the factor would set the weights apart from the masses, which come
+                    // from rounded scores, and from 2^32 on leave fp32.
+                    const bool fused = fabsf(ref) < 128.0f;
+                    const float x = s[nt][i], y = s[nt][2 + i], f = qf[nt][i];
+                    p[nt][i] = where0 >= 0 ? fast_exp2(fused ? __fmaf_rn(x, f, -ref) : __fsub_rn(__fmul_rn(x, f), ref)) : 0.0f;
+                    p[nt][2 + i] = where1 >= 0 ? fast_exp2(fused ? __fmaf_rn(y, f, -ref) : __fsub_rn(__fmul_rn(y, f), ref)) : 0.0f;
                     l[nt][i] += p[nt][i] + p[nt][2 + i];
                     p[nt][i] *= p_scale<T>();
                     p[nt][2 + i] *= p_scale<T>();

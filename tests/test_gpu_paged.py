@@ -225,6 +225,54 @@ def test_attention_cache_magnitudes(cuda, kv, k_size, v_size):
 
 
 @pytest.mark.parametrize("kv", ["f32", "f16", "bf16"])
+def test_attention_type_extremes(cuda, kv):
+    """The type's largest value in every element of K, of either sign by position: scores of fp32's size or beyond give
+    the positive positions all the weight; V at the largest value that a mean of 40 leaves in range."""
+    c = Cache(cuda, kv, 16, 2, 128, 16, [40, 5], seed=42, mass=False)
+    top = cuda.finfo(c.k.dtype).max
+    want = []
+    for i in range(2):
+        j, p, s = c.places(i)
+        sign = np.where(j % 3 == 1, 1.0, -1.0)
+        c.k[c.dev(p).long(), c.dev(s).long()] = (c.dev(sign)[:, None, None] * top).to(c.k.dtype)
+        want.append(c.v[c.dev(p[sign > 0]).long(), c.dev(s[sign > 0]).long()].double().mean(0))
+    q = cuda.full((2, 2048), 2.0 ** -3, device="cuda")
+    got = c.attend(q, scale=2.0 ** -5).double().view(2, 2, 8, 128)   # scores of +-top / 2: 128 * 2^-8 of it
+    for i in range(2):
+        assert bool((got[i] - want[i][:, None]).abs().max() <= 64 * U * c.v.double().abs().max())
+
+
+@pytest.mark.parametrize("kv", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("size", [1e5, 1e7, 1e9, 1e12, 1e25])
+def test_attention_huge_scores(cuda, kv, size):
+    """Where the largest score leads by more than its rounding (and 40: e^-40 < 2^-57), it takes all the weight and all
+    of the mass, however large the scores are."""
+    c = Cache(cuda, kv, 16, 2, 128, 16, [300, 77, 1], seed=44)
+    q = size * cuda.randn(3, 2048, device="cuda")
+    k, v = c.host()
+    before = c.mass.double().cpu().numpy()
+    got = c.attend(q).double().cpu().numpy().reshape(3, 16, 128)
+    qq, seen, add = q.double().cpu().numpy().reshape(3, 16, 128), 0, np.zeros_like(before)
+    for i in range(3):
+        j, p, s = c.places(i)
+        for h in range(16):
+            kk = k[p, s, h // 8]
+            sc = kk @ qq[i, h] * 128 ** -0.5
+            ds = 8 * np.sqrt(128) * U * 128 ** -0.5 * (np.abs(kk) @ np.abs(qq[i, h])).max()
+            top = sc.argmax()
+            if j.size == 1 or sc[top] - np.delete(sc, top).max() > 40 + 2 * ds:
+                seen += 1
+                assert np.allclose(got[i, h], v[p, s, h // 8][top], rtol=8 * U, atol=8 * U)
+                add[p[top], h // 8, s[top]] += 1
+            else:
+                add[p, h // 8, s] = np.nan   # undecided
+    assert seen > 40
+    m = c.mass.double().cpu().numpy()
+    decided = ~np.isnan(add)
+    assert np.isfinite(m).all() and np.all(np.abs(m - before - add)[decided] <= 64 * U * (before + 8)[decided])
+
+
+@pytest.mark.parametrize("kv", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")])
 def test_attention_values_that_are_not_finite_stay_in_their_head(cuda, kv, bad):
     """One infinite or NaN element of K or of V at a visible position: other KV heads, other sequences and, for V, other
