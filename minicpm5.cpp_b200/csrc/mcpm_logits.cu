@@ -6,7 +6,9 @@
 #include <cooperative_groups.h>
 
 #include "../../include/mcpm.h"
+#include "mcpm_cluster.h"
 #include "mcpm_device.cuh"
+#include "mcpm_paged.cuh"
 
 namespace mcpm {
 namespace {
@@ -284,17 +286,24 @@ __global__ void __launch_bounds__(LG_THREADS, 4) k_logits(const mcpm_logits_para
 
 using Kernel = void (*)(mcpm_logits_params);
 
-// The kernel of a variant, its attributes set once per device (setting them again does no harm).
+constexpr size_t LG_SMEM = LG_CHUNKS * LG_CHUNK * sizeof(uint16_t);
+
+// The kernel of a variant, its attributes set once per device (setting them again does no harm); null: the device
+// cannot run its cluster.
 template <int VEC, int BITS, bool LISTS, bool MASK>
 cudaError_t prepared(int dev, Kernel& kernel) {
-    static bool done[64] = {};
+    static signed char done[64] = {};   // 1: runs, -1: does not
     kernel = k_logits<VEC, LISTS, MASK, BITS>;
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    if (done[dev]) return cudaSuccess;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LG_CHUNKS * LG_CHUNK * static_cast<int>(sizeof(uint16_t)));
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    done[dev] = e == cudaSuccess;
-    return e;
+    if (!done[dev]) {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(LG_SMEM));
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return e;
+        const auto active = [&](int width) { return active_clusters(kernel, width, LG_THREADS, LG_SMEM); };
+        done[dev] = widest_cluster(1 << BITS, active) == 1 << BITS ? 1 : -1;
+    }
+    if (done[dev] < 0) kernel = nullptr;
+    return cudaSuccess;
 }
 template <int VEC, int BITS>
 cudaError_t pick(bool lists, bool mask, int dev, Kernel& kernel) {
@@ -325,16 +334,19 @@ extern "C" mcpm_status mcpm_logits_process(const mcpm_logits_params* params, voi
     if (p.allow && p.allow_stride < mask_words) return MCPM_BAD_ARG;
     auto aligned = [&](const float* q, int64_t stride) { return (reinterpret_cast<uintptr_t>(q) & 15u) == 0 && (p.n_seq == 1 || stride % 4 == 0); };
     const bool lists = p.hist || p.bias_token, mask = p.allow != nullptr;
-    const bool wide = static_cast<long long>(p.n_seq) << LG_WIDE_BITS <= 128;   // 148 SMs
     const bool vec = aligned(p.logits, p.logits_stride) && aligned(p.out, p.out_stride);
-    const int bits_cta = wide ? LG_WIDE_BITS : LG_CLUSTER_BITS;
-    const size_t smem = lists ? slice_chunks(p.n_vocab, bits_cta) * LG_CHUNK * sizeof(uint16_t) : 0;
-    int dev = 0;
+    int dev = 0, n_sm = 0;
     Kernel kernel = nullptr;
     cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess)
-        e = wide ? (vec ? pick<4, LG_WIDE_BITS>(lists, mask, dev, kernel) : pick<1, LG_WIDE_BITS>(lists, mask, dev, kernel))
-                 : (vec ? pick<4, LG_CLUSTER_BITS>(lists, mask, dev, kernel) : pick<1, LG_CLUSTER_BITS>(lists, mask, dev, kernel));
+    if (e == cudaSuccess) e = sm_count(dev, n_sm);
+    int bits_cta = LG_WIDE_BITS;
+    if (e == cudaSuccess && static_cast<long long>(p.n_seq) << LG_WIDE_BITS <= cluster_ctas(n_sm))
+        e = vec ? pick<4, LG_WIDE_BITS>(lists, mask, dev, kernel) : pick<1, LG_WIDE_BITS>(lists, mask, dev, kernel);
+    if (e == cudaSuccess && !kernel) {
+        bits_cta = LG_CLUSTER_BITS;
+        e = vec ? pick<4, LG_CLUSTER_BITS>(lists, mask, dev, kernel) : pick<1, LG_CLUSTER_BITS>(lists, mask, dev, kernel);
+    }
+    const size_t smem = lists ? slice_chunks(p.n_vocab, bits_cta) * LG_CHUNK * sizeof(uint16_t) : 0;
     if (e == cudaSuccess) {
         const unsigned cluster = 1u << bits_cta;
         cudaLaunchConfig_t cfg = {};

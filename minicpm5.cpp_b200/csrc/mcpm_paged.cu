@@ -7,6 +7,7 @@
 #include <cooperative_groups.h>
 
 #include "../../include/mcpm.h"
+#include "mcpm_cluster.h"
 #include "mcpm_device.cuh"
 #include "mcpm_paged.cuh"
 
@@ -87,7 +88,7 @@ struct EvictArgs {
     int n_keep, n_sink, n_recent;
 };
 
-constexpr int EV_MAX_CLUSTER = 16;   // beyond the portable 8: one GPC's SMs
+constexpr int EV_MAX_CLUSTER = 16;   // beyond the portable 8, where the device can run it
 constexpr int EV_BITS = 11, EV_BINS = 1 << EV_BITS, EV_PASSES = 3;   // digits of 11, 11 and 10 bits, highest first
 constexpr int EV_KEYS = 32768;   // keys a CTA holds in shared memory
 constexpr int EV_RANKED = 512;   // at most a CTA's threads
@@ -372,30 +373,36 @@ cudaError_t launch_evict_copy(const PagedGeom& g, const EvictArgs& a, int n_seq,
     return launch_dependent(g.head_dim == 64 ? k_paged_evict_copy<T, 64> : k_paged_evict_copy<T, 128>, grid, 32 * EV_COPY_WARPS, 0, s, g, a);
 }
 
-// One CTA for up to 3072 positions, more where the table has room for longer sequences and SMs are free (8000
+// One CTA for up to 3072 positions, more where the table has room for longer sequences (the lengths are the device's,
+// the host does not know them) and SMs are free (8000
 // positions: one CTA 16.6 us with the copy, two 15.5, four 13.3; 2112: one 11.4, two 12.3); CTAs of
 // 512 threads, two to an SM, where there are more pairs than SMs (200 pairs of 2621 positions: a second wave of
 // selections cost 9 us).
 template <int THREADS>
-cudaError_t prepare_select(int dev) {
-    static bool prepared[64] = {};
+cudaError_t prepare_select(int dev, int& widest) {   // per device: a repeated call finds the same again
+    static int known[64] = {};
     if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    if (prepared[dev]) return cudaSuccess;
-    cudaError_t e = cudaFuncSetAttribute(k_paged_evict_select<THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_SMEM);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(k_paged_evict_select<THREADS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    prepared[dev] = e == cudaSuccess;
-    return e;
+    if (!known[dev]) {
+        auto* kernel = k_paged_evict_select<THREADS>;
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_SMEM);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return e;
+        known[dev] = widest_cluster(EV_MAX_CLUSTER, [&](int width) { return active_clusters(kernel, width, THREADS, EV_SMEM); });
+    }
+    widest = known[dev];
+    return cudaSuccess;
 }
 cudaError_t launch_evict_select(const PagedGeom& g, const EvictArgs& a, int n_seq, cudaStream_t s) {
-    int dev = 0;
+    int dev = 0, n_sm = 0, widest = 0;
     cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = sm_count(dev, n_sm);
     if (e != cudaSuccess) return e;
     const long long room = static_cast<long long>(g.max_pages) * g.page_size, pairs = static_cast<long long>(n_seq) * g.n_head_kv;
-    const bool many = pairs > 148;   // SMs
-    e = many ? prepare_select<512>(dev) : prepare_select<1024>(dev);
+    const bool many = pairs > n_sm;
+    e = many ? prepare_select<512>(dev, widest) : prepare_select<1024>(dev, widest);
     if (e != cudaSuccess) return e;
     int cluster = 1;
-    while (cluster < EV_MAX_CLUSTER && cluster * 3072LL < room && pairs * cluster * 2 <= 128) cluster *= 2;
+    while (cluster < widest && cluster * 3072LL < room && pairs * cluster * 2 <= cluster_ctas(n_sm)) cluster *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(g.n_head_kv * cluster, n_seq);
     cfg.blockDim = dim3(many ? 512 : 1024);

@@ -67,6 +67,38 @@ __device__ __forceinline__ void kv_store4(__nv_bfloat16* p, float4 x) {
     *reinterpret_cast<uint2*>(p) = *reinterpret_cast<uint2*>(h);
 }
 
+// SMs of a device, asked for once.
+inline cudaError_t sm_count(int dev, int& n) {
+    static int known[64] = {};
+    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+    if (!known[dev]) {
+        int x = 0;
+        const cudaError_t e = cudaDeviceGetAttribute(&x, cudaDevAttrMultiProcessorCount, dev);
+        if (e != cudaSuccess) return e;
+        known[dev] = x;
+    }
+    n = known[dev];
+    return cudaSuccess;
+}
+// Clusters of `width` CTAs of a kernel that can run at once; -1: the device does not take such a launch.
+template <typename... P>
+int active_clusters(void (*kernel)(P...), int width, int threads, size_t smem) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(width);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = width;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess) return n;
+    cudaGetLastError();   // an answer, not a fault of the call that asked
+    return -1;
+}
+
 // Launches a kernel that may begin while the one before it in the stream ends (programmatic dependent launch).
 // The kernel calls grid_dep_wait in every CTA before it touches memory, so streams keep their order; what
 // overlaps is the launch itself, 1 to 2 us of a call of 5 to 10 us.

@@ -855,17 +855,10 @@ size_t paged_attention_workspace(const PagedGeom& g, int max_seqs) {
 cudaError_t launch_paged_attention(const PagedGeom& g, int kv_type, int max_seqs, const void* kc, const void* vc, float* mass,
                                    const int* table, const int* len, int n_seq, const float* q, long long q_stride, float* out,
                                    float scale, void* ws, cudaStream_t s) {
-    static int n_sms[64] = {};
-    int dev = 0;
+    int dev = 0, n_sm = 0;
     cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = sm_count(dev, n_sm);
     if (e != cudaSuccess) return e;
-    if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
-    if (!n_sms[dev]) {
-        int n = 0;
-        e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-        if (e != cudaSuccess) return e;
-        n_sms[dev] = n;
-    }
     uint8_t* w = static_cast<uint8_t*>(ws);
     AttArgs a{kc, vc, table, len, q, q_stride, out, scale, n_seq, g.n_head / g.n_head_kv};
     a.cnt = reinterpret_cast<unsigned*>(w);
@@ -875,9 +868,9 @@ cudaError_t launch_paged_attention(const PagedGeom& g, int kv_type, int max_seqs
     a.part = reinterpret_cast<float*>(w);
     w += up(sizeof(float) * part_floats(g));
     a.scores = reinterpret_cast<float*>(w);
-    if (kv_type == MCPM_KV_F32) return pick<float>(g, a, mass, dev, n_sms[dev], s);
-    if (kv_type == MCPM_KV_F16) return pick<__half>(g, a, mass, dev, n_sms[dev], s);
-    return pick<__nv_bfloat16>(g, a, mass, dev, n_sms[dev], s);
+    if (kv_type == MCPM_KV_F32) return pick<float>(g, a, mass, dev, n_sm, s);
+    if (kv_type == MCPM_KV_F16) return pick<__half>(g, a, mass, dev, n_sm, s);
+    return pick<__nv_bfloat16>(g, a, mass, dev, n_sm, s);
 }
 
 }  // namespace mcpm

@@ -103,3 +103,14 @@ def test_rope_table():
     buf = np.zeros(8, np.float32)
     for n, d, base in ((0, 2, 1e4), (4, 3, 1e4), (4, 0, 1e4), (4, 2, 0.0), (4, 2, float("nan"))):
         assert lib.mcpm_rope_table(E._fptr(buf), n, d, base) == E.BAD_ARG
+
+
+def test_cluster_width_rules(tmp_path):
+    """Clusters of 16 CTAs where the device can run one, of the portable 8 elsewhere, and no question asked up to 8."""
+    import os
+    import subprocess
+    from conftest import PKG, REPO
+    exe = str(tmp_path / "cluster_width")
+    subprocess.run(["g++", "-std=c++17", "-I", os.path.join(PKG, "csrc"), os.path.join(REPO, "tests", "cpp", "cluster_width.cpp"), "-o", exe], check=True)
+    out = subprocess.run([exe], capture_output=True, text=True, check=True).stdout
+    assert [int(x) for x in out.split()] == [16, 8, 8, 8, 1, 3, 130, 116, 7]
