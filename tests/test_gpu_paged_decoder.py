@@ -258,3 +258,38 @@ def test_a_conversation_outlives_its_rope_table(cuda, parity):
 
     a, b = run(4), run(64)
     assert a[0] == b[0] and np.array_equal(a[1], b[1]) and np.array_equal(a[2], b[2])
+
+
+@pytest.mark.gpu
+def test_an_evicting_step_keeps_the_heaviest_of_every_layer(cuda, parity):
+    """Masses and rows before a step that evicts name the positions that it keeps: K, V and masses of each layer and KV
+    head afterwards, the masses with what the step itself added."""
+    from test_gpu_paged import expected_kept
+    from mcpm import paged, synth
+    _, _, path = parity
+    d = paged.PagedDecoder(path, n_pages=8, max_positions=64, keep=30, slack=10, sink=2, recent=8)
+    s = d.open()
+    evictions = 0
+    for t in synth.prompt_ids(75, seed=21):
+        n = int(d.length[s])
+        if n < 40:
+            d.step({s: int(t)})
+            continue
+        evictions += 1
+        page, slot = d.table[s, np.arange(n) // 16].astype(np.int64), np.arange(n) % 16
+        k, v, m = (x.cpu().numpy() for x in (d.k, d.v, d.mass))
+        d.step({s: int(t)})
+        to, at = d.table[s, np.arange(31) // 16].astype(np.int64), np.arange(31) % 16
+        k2, v2, m2 = (x.cpu().numpy() for x in (d.k, d.v, d.mass))
+        for layer in range(d.n_layer):
+            for h in range(2):
+                mass = m[layer, page, h, slot]
+                kept = expected_kept(mass, np.arange(n), n, 30, 2, 8)
+                assert np.array_equal(k2[layer, to[:30], at[:30], h], k[layer, page[kept], slot[kept], h])
+                assert np.array_equal(v2[layer, to[:30], at[:30], h], v[layer, page[kept], slot[kept], h])
+                now = m2[layer, to, h, at]
+                assert np.all(now[:30] >= mass[kept])   # the step adds weights, none below zero
+                added = now.astype(np.float64).sum() - mass[kept].astype(np.float64).sum()
+                assert abs(added - 8) < 1e-4            # eight heads' weights, over 31 positions, on masses of at most 300
+        assert d.length[s] == 31
+    assert evictions >= 3

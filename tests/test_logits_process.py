@@ -163,6 +163,29 @@ def test_logits_ties_and_dead_ends(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,v", [(1, 32768), (8, 5001), (9, 5001), (9, 32768), (20, 130560), (64, 8192)])
+@pytest.mark.parametrize("hist,bias", [(0, 0), (60, 0), (0, 9), (700, 40)])
+@pytest.mark.parametrize("mask", [False, True])
+def test_logits_variants(cuda, n, v, hist, bias, mask):
+    """Rows of sixteen and of eight CTAs, aligned and odd ones, with and without lists and masks."""
+    Rows(cuda, n, v, hist, bias, mask, seed=n + v + hist).check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v", [5001, 130560])
+def test_logits_do_not_depend_on_the_rows_beside_them(cuda, v):
+    """A row alone, among few and among many rows: the same bits, whatever the number of CTAs that share it."""
+    r = Rows(cuda, 30, v, 300, 20, True, seed=v)
+    all_rows, tokens = r.run()
+    for n in (1, 8, 9):
+        few = Rows(cuda, n, v, 300, 20, True, seed=v)
+        for k in ("x", "hist", "hist_len", "pen", "bias_token", "bias", "bias_len", "allow"):
+            setattr(few, k, getattr(r, k)[:n])
+        got, token = few.run()
+        assert np.array_equal(got, all_rows[:n]) and np.array_equal(token, tokens[:n])
+
+
+@pytest.mark.gpu
 def test_logits_on_a_side_stream_and_in_a_graph(cuda):
     from mcpm import engine as E
     r = Rows(cuda, 3, 9001, 40, 3, True, seed=5)
