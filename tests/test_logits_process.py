@@ -186,6 +186,23 @@ def test_logits_do_not_depend_on_the_rows_beside_them(cuda, v):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [2, 12])
+def test_logits_without_the_greedy_token(cuda, n):
+    """The same rows where no greedy token is asked for, whose cluster has nothing to exchange."""
+    from mcpm import engine as E
+    r = Rows(cuda, n, 9001, 200, 5, True, seed=n)
+    want, _ = r.run()
+    d = {k: cuda.from_numpy(getattr(r, k).view(np.int32) if k == "allow" else getattr(r, k)).cuda()
+         for k in ("x", "hist", "hist_len", "pen", "bias_token", "bias", "bias_len", "allow")}
+    out = cuda.zeros(n, 9001, device="cuda")
+    E.logits_process(d["x"].data_ptr(), out.data_ptr(), n, 9001, hist=d["hist"].data_ptr(), hist_stride=200, hist_len=d["hist_len"].data_ptr(),
+                     penalties=d["pen"].data_ptr(), bias_token=d["bias_token"].data_ptr(), bias=d["bias"].data_ptr(), bias_stride=5,
+                     bias_len=d["bias_len"].data_ptr(), allow=d["allow"].data_ptr())
+    cuda.cuda.synchronize()
+    assert np.array_equal(out.cpu().numpy(), want)
+
+
+@pytest.mark.gpu
 def test_logits_on_a_side_stream_and_in_a_graph(cuda):
     from mcpm import engine as E
     r = Rows(cuda, 3, 9001, 40, 3, True, seed=5)
