@@ -366,7 +366,7 @@ mcpm_status mcpm_paged_append(const mcpm_paged_config* cfg, const mcpm_paged_poo
  * sequence that sees none gets zeros.  q and out: rows of n_head * head_dim floats, q_stride floats
  * between the rows of q (0: packed).  scale 0: 1/sqrt(head_dim).  With pool->mass, each visible
  * position's mass grows by the sum of its weights over the g query heads of its KV head; the
- * sequences of such a call share no pages.  Scores, and sums of exp(score - largest score) |V|, are held
+ * sequences of such a call share no pages, and none names a page twice.  Scores, and sums of exp(score - largest score) |V|, are held
  * in fp32: K and V may be as large as their type allows where these stay below 2e38.  K and V of the
  * visible positions are finite; where one is not, outputs and masses of its KV head in that sequence may be
  * NaN, and nothing else is touched.  Results do not depend on how the work was split over
@@ -381,7 +381,8 @@ mcpm_status mcpm_paged_attention(const mcpm_paged_config* cfg, const mcpm_paged_
  * prefix pages of other sequences stay valid and the caller frees its own.  kept (int32
  * [n_seq][n_head_kv][n_keep]) receives the positions, -1 beyond the last; new_len (int32 [n_seq]) the
  * number kept: n_keep, or all present positions where they are fewer.  No page of dst_table may be
- * one that a row of table names.  n_sink + n_recent <= n_keep <= max_pages * page_size. */
+ * one that a row of table names, and it names none twice.  n_sink + n_recent <= n_keep <= max_pages *
+ * page_size.  ws is checked as in the attention and reserved: nothing is kept in it. */
 mcpm_status mcpm_paged_evict(const mcpm_paged_config* cfg, const mcpm_paged_pool* pool, const int* table,
                              const int* seq_len, const int* dst_table, int* new_len, int* kept, int n_seq, int n_keep,
                              int n_sink, int n_recent, void* ws, size_t ws_bytes, void* stream);

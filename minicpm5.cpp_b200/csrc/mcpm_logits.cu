@@ -50,9 +50,9 @@ __device__ __forceinline__ void take(Best& a, const Best& b) {
 // largest index is the last entry).  The streaming pass puts the logits of listed tokens aside, and they are
 // computed side by side after it.  A slice with more listed tokens than the list holds is cut in half until
 // they fit.  VEC = 4 where all rows are 16-byte aligned, else 1.
-// 64 rows of 130560 without lists 13.5 us, 5.0 TB/s (a device copy of them: 16 us); with 4096 tokens of history,
-// 64 biases and a mask each 24.6 us, of which 10.7 us are bytes: the lists' round trips come before the logits'.
-// One row 6.5 us.
+// 64 rows of 130560 without lists 13.4 us, 5.0 TB/s (a device copy of them: 16 us); with 4096 tokens of history,
+// 64 biases and a mask each 24.8 us, of which 10.7 us are bytes: the lists' round trips come before the logits'.
+// One row 6.4 us.
 template <int VEC, bool LISTS, bool MASK, int bits_cta>
 __global__ void __launch_bounds__(LG_THREADS, 4) k_logits(const mcpm_logits_params p) {
     extern __shared__ __align__(16) uint16_t words[];    // [tokens of a slice] place on the list plus 1; zero: not listed

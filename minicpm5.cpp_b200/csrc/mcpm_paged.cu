@@ -1,5 +1,5 @@
-// Paged KV cache: append of new tokens (RoPE, rounding, page writes), attention of one new token
-// per sequence over its pages, and eviction of the positions with the least attention mass.
+// Paged KV cache: append of new tokens (RoPE, rounding, page writes) and eviction of the positions with
+// the least attention mass; the attention between them is in mcpm_paged_attention.cu.
 #include <algorithm>
 #include <cmath>
 #include <cstdio>
@@ -26,7 +26,7 @@ struct AppendArgs {
 // A CTA per token; a token's rows are its query heads, its KV heads' K, then their V.  D / 4 lanes to a row, a
 // float4 (two rotary pairs, the same ones in every row) a lane, AP_HELD rows of a lane in flight.
 // (x0, x1) -> (c x0 - s x1, s x0 + c x1), one fma per output as mcpm_rope_kv_append.
-// Bound by the memory: 8192 tokens of 16 + 2 + 2 heads x 128 (fp32 cache) 30.5 us, 5.6 TB/s; 64 tokens 5.0 us, the
+// Bound by the memory: 8192 tokens of 16 + 2 + 2 heads x 128 (fp32 cache) 30.5 us, 5.6 TB/s; 64 tokens 5.3 us, the
 // time of a call.
 constexpr int AP_WARPS = 4, AP_HELD = 5;
 template <typename T, int D>

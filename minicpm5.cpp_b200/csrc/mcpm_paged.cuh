@@ -1,4 +1,4 @@
-// Geometry of a paged KV pool as the kernels of mcpm_paged.cu see it: which element row a
+// Geometry of a paged KV pool as the kernels of mcpm_paged.cu and mcpm_paged_attention.cu see it: which element row a
 // position of a sequence lies in, with page ids and positions from device memory that are
 // checked before anything is addressed through them.
 #pragma once
@@ -100,8 +100,9 @@ int active_clusters(void (*kernel)(P...), int width, int threads, size_t smem) {
 }
 
 // Launches a kernel that may begin while the one before it in the stream ends (programmatic dependent launch).
-// The kernel calls grid_dep_wait in every CTA before it touches memory, so streams keep their order; what
-// overlaps is the launch itself, 1 to 2 us of a call of 5 to 10 us.
+// The kernel calls grid_dep_wait in every CTA before it touches memory that the kernel before it may write, so streams
+// keep their order; what overlaps is the launch itself, 1 to 2 us of a call of 5 to 10 us.  (One kernel reads before
+// its wait: the eviction's copy, a table that was final before the selection in front of it began.)
 template <typename... P, typename... A>
 cudaError_t launch_dependent(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t s, const A&... args) {
     cudaLaunchConfig_t cfg = {};

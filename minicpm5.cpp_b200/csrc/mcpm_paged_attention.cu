@@ -17,10 +17,11 @@
 // row, an equal share per CTA.  A pair that spans several CTAs leaves a partial result per CTA, and the
 // CTA that arrives last joins them in order of position, so results do not depend on arrival order.
 //
-// Measured (16 query heads, 2 KV heads, 128 dims): 4 x 131072 positions of fp16 93 us, 5.8 TB/s; of fp32 171 us,
-// 6.3 TB/s; bound by the memory (a device copy: 6.46 TB/s).  Short calls are bound by a chain of round trips:
-// lengths, page table, K, V, then record, arrival and join where a pair is split: 8193 fp32 positions 13.7 us,
-// of which 2.6 us are bytes; 137 positions 8.7 us.
+// Measured (16 query heads, 2 KV heads, 128 dims): 4 x 131072 positions of fp16 95 us, 5.7 TB/s; of fp32 181 us,
+// 5.9 TB/s; bound by the memory (a device copy: 6.46 TB/s).  Short calls are bound by a chain of round trips:
+// lengths, page table, K, V, then record, arrival and join where a pair is split: 8193 fp32 positions 13.6 us,
+// of which 2.6 us are bytes; 137 positions 8.7 us.  With one KV head, whose 16 heads take two products a tile,
+// 4 x 131072 fp16 positions take 65 us, 4.1 TB/s: eight warps an SM carry twice the products.
 #include <algorithm>
 #include <cmath>
 
@@ -356,8 +357,8 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
 #pragma unroll 1
     for (int i = 0; i < L::SLOTS - 1; ++i) issue(i, i);
 
-    // ---- A pair of several CTAs leaves a record (m, l, o) per CTA.  Records are joined eight at a time, in order
-    // of position, by the CTA that arrives last at the eight; its result is a record of the next level, and the
+    // ---- A pair of several CTAs leaves a record (m, l, o) per CTA.  Records are joined FAN at a time, in order
+    // of position, by the CTA that arrives last at them; its result is a record of the next level, and the
     // last level's is the output.  One CTA reading all records of a long sequence took 7 us of a 20 us call.
     const int rec = 2 * PAGED_MAX_GROUP + group * D;   // floats of a record
     auto arrive = [&](int level, int slot, int members) {   // thread 0, after the CTA's stores and a barrier
@@ -376,7 +377,7 @@ __global__ void __launch_bounds__(THREADS, Tile<T, D, NT>::CTAS) k_paged_attenti
         const int step = 1 << FAN_BITS * level, at = s.k >> FAN_BITS * (level + 1) << FAN_BITS * (level + 1);
         return min(FAN, (s.np - at + step - 1) >> FAN_BITS * level);
     };
-    auto join = [&](Shared s) {   // s_last: whether this CTA arrived last at its first eight
+    auto join = [&](Shared s) {   // s_last: whether this CTA arrived last at its first FAN records
         for (int level = 0; s_last; ++level) {
             const int at = s.k >> FAN_BITS * (level + 1) << FAN_BITS * (level + 1), members = members_of(s, level);
             const bool done = s.np <= 1 << FAN_BITS * (level + 1);
